@@ -1,0 +1,247 @@
+// mx_quantize.cu -- block quantisation to the microscaled formats, reading back, and the re-layout
+// of scales.
+#include "mx_common.cuh"
+
+namespace s24 {
+
+using namespace mx;
+
+constexpr int kQuantThreads = 256;
+
+__device__ __forceinline__ uint4 load16(const void* p)
+{
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+
+// One thread per block of 32 elements; four neighbouring threads share a 128-column chunk and put its
+// scales together into the one word that tensor-core order keeps together.  With TC the index space
+// covers whole 128 x 128 records, and threads outside the matrix only write the filler scale 0.
+template <int DT, int FMT, bool TC>
+__global__ void __launch_bounds__(kQuantThreads)
+mx_quantize_kernel(const uint8_t* __restrict__ x, uint32_t R, uint32_t KB, uint32_t KB_pad, uint32_t total, int64_t row_bytes,
+                   uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, uint8_t* __restrict__ scales_tc)
+{
+    constexpr int kElem = DT == S24_FP32 ? 4 : 2;
+    const uint32_t t = blockIdx.x * kQuantThreads + threadIdx.x;
+    const uint32_t r = t / KB_pad, kb = t - r * KB_pad;
+    uint32_t s = 0;
+    if (t < total && r < R && kb < KB) {
+        const uint8_t* src = x + (int64_t)r * row_bytes + (int64_t)kb * (kBlock * kElem);
+        float v[kBlock];
+#pragma unroll
+        for (int i = 0; i < 2 * kElem; ++i) {
+            const uint4 w = load16(src + 16 * i);
+            const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if constexpr (DT == S24_FP32) {
+                    v[4 * i + j] = __uint_as_float(u[j]);
+                } else {
+                    const float2 f = unpack2<DT>(u[j]);
+                    v[8 * i + 2 * j] = f.x;
+                    v[8 * i + 2 * j + 1] = f.y;
+                }
+            }
+        }
+        uint32_t amax = 0;
+#pragma unroll
+        for (int i = 0; i < kBlock; ++i) amax = max(amax, magnitude_bits(v[i]));
+        s = scale_code<FMT>(amax);
+        const float up = scale_up(s);
+#pragma unroll
+        for (int i = 0; i < kBlock; ++i) v[i] *= up;
+        uint32_t c[Format<FMT>::kBytes / 4];
+        encode_block<FMT>(v, s != 255u, c);
+        const int64_t at = (int64_t)r * KB + kb;
+        uint4* dst = reinterpret_cast<uint4*>(codes + at * Format<FMT>::kBytes);
+#pragma unroll
+        for (int i = 0; i < Format<FMT>::kBytes / 16; ++i) dst[i] = make_uint4(c[4 * i], c[4 * i + 1], c[4 * i + 2], c[4 * i + 3]);
+        if (scales != nullptr) scales[at] = (uint8_t)s;
+    }
+    if constexpr (TC) {
+        uint32_t word = s << (8 * (threadIdx.x & 3));
+        word |= __shfl_xor_sync(0xFFFFFFFFu, word, 1);
+        word |= __shfl_xor_sync(0xFFFFFFFFu, word, 2);
+        if (t < total && (threadIdx.x & 3) == 0) *reinterpret_cast<uint32_t*>(scales_tc + tc_offset(r, kb, KB_pad >> 2)) = word;
+    }
+}
+
+// One thread per block.
+template <int DT, int FMT>
+__global__ void __launch_bounds__(kQuantThreads)
+mx_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int tc, uint32_t KB, uint32_t total,
+                     uint8_t* __restrict__ out)
+{
+    constexpr int kElem = DT == S24_FP32 ? 4 : 2;
+    const uint32_t t = blockIdx.x * kQuantThreads + threadIdx.x;
+    if (t >= total) return;
+    const uint32_t r = t / KB, kb = t - r * KB;
+    const float s = scale_value(scales[tc ? tc_offset(r, kb, (KB + 3) / 4) : (int64_t)t]);
+    const uint8_t* src = codes + (int64_t)t * Format<FMT>::kBytes;
+    float v[kBlock];
+#pragma unroll
+    for (int i = 0; i < Format<FMT>::kBytes / 16; ++i) {
+        const uint4 w = load16(src + 16 * i);
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if constexpr (FMT == S24_MXFP4) {
+                from_e2m1x4(u[j] & 0xFFFFu, &v[8 * j]);
+                from_e2m1x4(u[j] >> 16, &v[8 * j + 4]);
+            } else {
+                from_e4m3x2(u[j] & 0xFFFFu, &v[16 * i + 4 * j]);
+                from_e4m3x2(u[j] >> 16, &v[16 * i + 4 * j + 2]);
+            }
+        }
+    }
+    uint4* dst = reinterpret_cast<uint4*>(out + (int64_t)t * (kBlock * kElem));
+#pragma unroll
+    for (int i = 0; i < 2 * kElem; ++i) {
+        uint32_t u[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if constexpr (DT == S24_FP32) u[j] = __float_as_uint(v[4 * i + j] * s);
+            else u[j] = mx::pack2<DT>(v[8 * i + 2 * j] * s, v[8 * i + 2 * j + 1] * s);
+        }
+        dst[i] = make_uint4(u[0], u[1], u[2], u[3]);
+    }
+}
+
+// One thread per scale of the destination; positions of tensor-core order outside the matrix get 0.
+template <bool TO_TC>
+__global__ void __launch_bounds__(kQuantThreads)
+mx_scales_convert_kernel(const uint8_t* __restrict__ src, uint8_t* __restrict__ dst, uint32_t R, uint32_t KB, uint32_t total)
+{
+    const uint32_t t = blockIdx.x * kQuantThreads + threadIdx.x;
+    if (t >= total) return;
+    const uint32_t chunks = (KB + 3) / 4;
+    if constexpr (TO_TC) {
+        const uint32_t rec = t >> 9, in = t & 511;
+        const uint32_t tile = rec / chunks, chunk = rec - tile * chunks;
+        const uint32_t r = tile * 128 + ((in >> 2) & 3) * 32 + (in >> 4), kb = chunk * 4 + (in & 3);
+        dst[t] = (r < R && kb < KB) ? src[(int64_t)r * KB + kb] : (uint8_t)0;
+    } else {
+        const uint32_t r = t / KB;
+        dst[t] = src[tc_offset(r, t - r * KB, chunks)];
+    }
+}
+
+// shape rules shared by the entry points; the index space of blocks has to fit 31 bits
+static int check_mx_shape(const char* who, int64_t R, int64_t K)
+{
+    if (R < 0 || K < 0 || K % kBlock != 0)
+        return fail(S24_ERR_SHAPE, "%s: needs R >= 0 and K a multiple of 32 (got R=%lld K=%lld)", who, (long long)R, (long long)K);
+    if (R > 0x7FFFFF00ll || K > 0x7FFFFF00ll || (K > 0 && row_tiles(R) * 128 > 0x7FFFFF00ll / (k_chunks(K) * 4)))
+        return fail(S24_ERR_SHAPE, "%s: %lld x %lld has too many blocks of 32", who, (long long)R, (long long)K);
+    return S24_OK;
+}
+
+template <int DT, int FMT>
+static void launch_quantize(const void* x, int64_t R, int64_t K, int64_t row_bytes, void* codes, void* scales, void* tc, cudaStream_t st)
+{
+    const uint32_t KB = (uint32_t)(K / kBlock);
+    const uint32_t KB_pad = tc ? (uint32_t)(k_chunks(K) * 4) : KB;
+    const uint32_t total = (uint32_t)(tc ? row_tiles(R) * 128 : R) * KB_pad;
+    const unsigned grid = (total + kQuantThreads - 1) / kQuantThreads;
+    auto* xs = static_cast<const uint8_t*>(x);
+    auto* c = static_cast<uint8_t*>(codes);
+    auto* s = static_cast<uint8_t*>(scales);
+    auto* t = static_cast<uint8_t*>(tc);
+    if (tc) mx_quantize_kernel<DT, FMT, true><<<grid, kQuantThreads, 0, st>>>(xs, (uint32_t)R, KB, KB_pad, total, row_bytes, c, s, t);
+    else mx_quantize_kernel<DT, FMT, false><<<grid, kQuantThreads, 0, st>>>(xs, (uint32_t)R, KB, KB_pad, total, row_bytes, c, s, t);
+}
+
+template <int DT, int FMT>
+static void launch_dequantize(const void* codes, const void* scales, int layout, void* out, int64_t R, int64_t K, cudaStream_t st)
+{
+    const uint32_t KB = (uint32_t)(K / kBlock), total = (uint32_t)R * KB;
+    mx_dequantize_kernel<DT, FMT><<<(total + kQuantThreads - 1) / kQuantThreads, kQuantThreads, 0, st>>>(
+        static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), layout == S24_SCALES_TC, KB, total, static_cast<uint8_t*>(out));
+}
+
+}  // namespace s24
+
+using namespace s24;
+
+extern "C" size_t s24_mx_scales_tc_bytes(int64_t R, int64_t K)
+{
+    if (R <= 0 || K <= 0) return 0;
+    return (size_t)row_tiles(R) * (size_t)k_chunks(K) * kRecordBytes;
+}
+
+extern "C" int s24_mx_quantize(const void* x, int64_t R, int64_t K, int64_t ld, int dtype, int fmt, void* codes, void* scales,
+                               void* scales_tc, void* stream)
+{
+    if (dtype != S24_FP16 && dtype != S24_BF16 && dtype != S24_FP32) return fail(S24_ERR_INVALID_ARG, "mx_quantize: bad dtype %d", dtype);
+    if (fmt != S24_MXFP4 && fmt != S24_MXFP8) return fail(S24_ERR_INVALID_ARG, "mx_quantize: bad format %d", fmt);
+    int rc = check_mx_shape("mx_quantize", R, K);
+    if (rc) return rc;
+    if (R == 0 || K == 0) return S24_OK;
+    if (x == nullptr || codes == nullptr || (scales == nullptr && scales_tc == nullptr))
+        return fail(S24_ERR_INVALID_ARG, "mx_quantize: null pointer");
+    const int64_t elem = dtype == S24_FP32 ? 4 : 2;
+    if (ld < K || ld > (INT64_MAX >> 2) / R || (ld * elem) % 16 != 0)
+        return fail(S24_ERR_SHAPE, "mx_quantize: the row stride must be >= K and a multiple of 16 bytes (got %lld elements)", (long long)ld);
+    if (!aligned(x, 16) || !aligned(codes, 16) || !aligned(scales_tc, 16))
+        return fail(S24_ERR_INVALID_ARG, "mx_quantize: pointers must be 16-byte aligned");
+    auto st = static_cast<cudaStream_t>(stream);
+    if (fmt == S24_MXFP4) {
+        if (dtype == S24_FP16) launch_quantize<S24_FP16, S24_MXFP4>(x, R, K, ld * elem, codes, scales, scales_tc, st);
+        else if (dtype == S24_BF16) launch_quantize<S24_BF16, S24_MXFP4>(x, R, K, ld * elem, codes, scales, scales_tc, st);
+        else launch_quantize<S24_FP32, S24_MXFP4>(x, R, K, ld * elem, codes, scales, scales_tc, st);
+    } else {
+        if (dtype == S24_FP16) launch_quantize<S24_FP16, S24_MXFP8>(x, R, K, ld * elem, codes, scales, scales_tc, st);
+        else if (dtype == S24_BF16) launch_quantize<S24_BF16, S24_MXFP8>(x, R, K, ld * elem, codes, scales, scales_tc, st);
+        else launch_quantize<S24_FP32, S24_MXFP8>(x, R, K, ld * elem, codes, scales, scales_tc, st);
+    }
+    return check_cuda(cudaGetLastError(), "mx_quantize launch");
+}
+
+extern "C" int s24_mx_dequantize(const void* codes, const void* scales, int layout, void* out, int64_t R, int64_t K, int fmt, int dtype,
+                                 void* stream)
+{
+    if (dtype != S24_FP16 && dtype != S24_BF16 && dtype != S24_FP32) return fail(S24_ERR_INVALID_ARG, "mx_dequantize: bad dtype %d", dtype);
+    if (fmt != S24_MXFP4 && fmt != S24_MXFP8) return fail(S24_ERR_INVALID_ARG, "mx_dequantize: bad format %d", fmt);
+    if (layout != S24_SCALES_ROWS && layout != S24_SCALES_TC) return fail(S24_ERR_INVALID_ARG, "mx_dequantize: bad layout %d", layout);
+    int rc = check_mx_shape("mx_dequantize", R, K);
+    if (rc) return rc;
+    if (R == 0 || K == 0) return S24_OK;
+    if (codes == nullptr || scales == nullptr || out == nullptr) return fail(S24_ERR_INVALID_ARG, "mx_dequantize: null pointer");
+    if (!aligned(codes, 16) || !aligned(out, 16)) return fail(S24_ERR_INVALID_ARG, "mx_dequantize: pointers must be 16-byte aligned");
+    auto st = static_cast<cudaStream_t>(stream);
+    if (fmt == S24_MXFP4) {
+        if (dtype == S24_FP16) launch_dequantize<S24_FP16, S24_MXFP4>(codes, scales, layout, out, R, K, st);
+        else if (dtype == S24_BF16) launch_dequantize<S24_BF16, S24_MXFP4>(codes, scales, layout, out, R, K, st);
+        else launch_dequantize<S24_FP32, S24_MXFP4>(codes, scales, layout, out, R, K, st);
+    } else {
+        if (dtype == S24_FP16) launch_dequantize<S24_FP16, S24_MXFP8>(codes, scales, layout, out, R, K, st);
+        else if (dtype == S24_BF16) launch_dequantize<S24_BF16, S24_MXFP8>(codes, scales, layout, out, R, K, st);
+        else launch_dequantize<S24_FP32, S24_MXFP8>(codes, scales, layout, out, R, K, st);
+    }
+    return check_cuda(cudaGetLastError(), "mx_dequantize launch");
+}
+
+extern "C" int s24_mx_scales_convert(const void* src, int from_layout, void* dst, int to_layout, int64_t R, int64_t K, void* stream)
+{
+    if ((from_layout != S24_SCALES_ROWS && from_layout != S24_SCALES_TC) || (to_layout != S24_SCALES_ROWS && to_layout != S24_SCALES_TC))
+        return fail(S24_ERR_INVALID_ARG, "mx_scales_convert: bad layout %d -> %d", from_layout, to_layout);
+    if (from_layout == to_layout) return fail(S24_ERR_UNSUPPORTED, "mx_scales_convert: source and destination layouts are the same");
+    int rc = check_mx_shape("mx_scales_convert", R, K);
+    if (rc) return rc;
+    if (R == 0 || K == 0) return S24_OK;
+    if (src == nullptr || dst == nullptr) return fail(S24_ERR_INVALID_ARG, "mx_scales_convert: null pointer");
+    auto st = static_cast<cudaStream_t>(stream);
+    auto* s = static_cast<const uint8_t*>(src);
+    auto* d = static_cast<uint8_t*>(dst);
+    const uint32_t KB = (uint32_t)(K / kBlock);
+    if (to_layout == S24_SCALES_TC) {
+        const uint32_t total = (uint32_t)s24_mx_scales_tc_bytes(R, K);
+        mx_scales_convert_kernel<true><<<(total + kQuantThreads - 1) / kQuantThreads, kQuantThreads, 0, st>>>(s, d, (uint32_t)R, KB, total);
+    } else {
+        const uint32_t total = (uint32_t)R * KB;
+        mx_scales_convert_kernel<false><<<(total + kQuantThreads - 1) / kQuantThreads, kQuantThreads, 0, st>>>(s, d, (uint32_t)R, KB, total);
+    }
+    return check_cuda(cudaGetLastError(), "mx_scales_convert launch");
+}

@@ -70,6 +70,8 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, int bf16)
 int make_map_2d(CUtensorMap* map, CUtensorMapDataType type, int elem_bytes, const void* base, uint64_t inner,
                 uint64_t outer, uint64_t row_stride_bytes, uint32_t box_inner, uint32_t box_outer,
                 CUtensorMapSwizzle swz, const char* what);
+int make_map_3d(CUtensorMap* map, CUtensorMapDataType type, const void* base, const uint64_t (&dims)[3],
+                const uint64_t (&stride_bytes)[2], const uint32_t (&box)[3], CUtensorMapSwizzle swz, const char* what);
 int* status_word_address();   // device address of the status word on the current device, or null
 
 }  // namespace s24

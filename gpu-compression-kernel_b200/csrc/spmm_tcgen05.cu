@@ -596,6 +596,19 @@ int make_map_2d(CUtensorMap* map, CUtensorMapDataType type, int elem_bytes, cons
     return S24_OK;
 }
 
+int make_map_3d(CUtensorMap* map, CUtensorMapDataType type, const void* base, const uint64_t (&dims)[3],
+                const uint64_t (&stride_bytes)[2], const uint32_t (&box)[3], CUtensorMapSwizzle swz, const char* what)
+{
+    EncodeTiledFn fn = encode_tiled();
+    if (fn == nullptr) return fail(S24_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+    const cuuint64_t d[3] = {dims[0], dims[1], dims[2]}, s[2] = {stride_bytes[0], stride_bytes[1]};
+    const cuuint32_t b[3] = {box[0], box[1], box[2]}, estr[3] = {1, 1, 1};
+    CUresult r = fn(map, type, 3, const_cast<void*>(base), d, s, b, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swz,
+                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(S24_ERR_CUDA, "cuTensorMapEncodeTiled(%s) failed with CUresult %d", what, (int)r);
+    return S24_OK;
+}
+
 struct GemmArgs {
     bool bt;   // B given transposed: (N, K) row-major, ldb = its row stride
     const void* vals;

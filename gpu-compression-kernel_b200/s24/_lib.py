@@ -17,6 +17,9 @@ INT8, INT32, FP32 = 2, 3, 4
 MODE_SIGNED, MODE_MAGNITUDE = 0, 1
 TIE_REFERENCE, TIE_LOWER, TIE_HIGHER = 0, 1, 2
 META_LOGICAL, META_REF, META_TC = 0, 1, 2
+MXFP4, MXFP8 = 0, 1
+SCALES_ROWS, SCALES_TC = 0, 1
+MX_NORM_MAX_K = 65536
 STATIC_SCRATCH_BYTES = 8 << 20
 PEER_HANDLE_BYTES = 64
 
@@ -47,6 +50,13 @@ SIGNATURES = {
                                   ctypes.POINTER(TileCfg), _vp]),
     "s24_spmm_prune_in": (_i32, [_vp, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i32, _i32, _i32, _vp]),
     "s24_spmm_scatter": (_i32, [_vp, _vp, _vp, ctypes.POINTER(_vp), _i32, _i64, _i64, _i64, _i64, _i64, _i32, _vp]),
+    "s24_mx_scales_tc_bytes": (_sz, [_i64, _i64]),
+    "s24_mx_quantize": (_i32, [_vp, _i64, _i64, _i64, _i32, _i32, _vp, _vp, _vp, _vp]),
+    "s24_mx_dequantize": (_i32, [_vp, _vp, _i32, _vp, _i64, _i64, _i32, _i32, _vp]),
+    "s24_mx_scales_convert": (_i32, [_vp, _i32, _vp, _i32, _i64, _i64, _vp]),
+    "s24_mx_rms_norm": (_i32, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, ctypes.c_double, _i32, _i32, _vp, _vp, _vp, _vp]),
+    "s24_mx_matmul": (_i32, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _i32, _i32,
+                             ctypes.POINTER(TileCfg), _vp]),
     "s24_peer_alloc": (_i32, [_sz, ctypes.POINTER(_vp)]),
     "s24_peer_free": (_i32, [_vp]),
     "s24_peer_export": (_i32, [_vp, _vp]),

@@ -1,0 +1,214 @@
+"""Microscaled formats: quantise, read back, multiply, and the norm that quantises its output.
+
+A quantised matrix is (codes, scales).  "mxfp4" codes are uint8, two elements to a byte (the even one in the
+low half); "mxfp8" codes are float8_e4m3fn.  Every 32 elements of the last dimension share a power of two,
+2^(scale - 127), held as uint8 in "rows" layout ((..., K / 32)) or in the order the tensor cores read ("tc",
+one flat buffer; include/s24.h gives both).  The product takes "tc"; "rows" is what checkpoints hold.
+
+Like the rest of the library these are inference calls: results carry no gradient.
+"""
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch
+
+from . import _lib as L
+from .ops import _after_gemm, _on_device, _p, _require_cuda, _stream, _tile_cfg
+
+_DT = {torch.float16: L.FP16, torch.bfloat16: L.BF16, torch.float32: L.FP32}
+_FMT = {"mxfp4": L.MXFP4, "mxfp8": L.MXFP8}
+_SCALES = {"rows": L.SCALES_ROWS, "tc": L.SCALES_TC}
+_SCALE_TYPES = (torch.uint8, torch.float8_e8m0fnu)
+
+
+def mx_scales_numel(R: int, K: int) -> int:
+    """bytes of a tensor-core-order scale buffer for an (R, K) matrix"""
+    return int(L.lib().s24_mx_scales_tc_bytes(R, K))
+
+
+def _rows_of(t: torch.Tensor) -> Tuple[int, int]:
+    if t.dim() < 1:
+        raise RuntimeError("expected a tensor of at least one dimension")
+    k = t.shape[-1]
+    r = 1
+    for n in t.shape[:-1]:
+        r *= n
+    return r, k
+
+
+def _matrix(t: torch.Tensor, R: int, step: int) -> Tuple[torch.Tensor, int]:
+    """t as (R, width) rows with unit column stride, whose pointer and row stride are multiples of `step` bytes
+    (copied if they are not), and the row stride in elements"""
+    width = t.shape[-1]
+    if t.dim() != 2:
+        t = t.reshape(R, width)
+    size = t.element_size()
+    stride = t.stride(0) if R > 1 else width
+    if t.stride(1) != 1 and width > 1 or stride < width or stride * size % step or t.data_ptr() % step:
+        t, stride = t.clone(memory_format=torch.contiguous_format), width
+    return t, stride
+
+
+def _check_fmt(fmt: str) -> int:
+    if fmt not in _FMT:
+        raise ValueError(f"unknown format {fmt!r} (have 'mxfp4' and 'mxfp8')")
+    return _FMT[fmt]
+
+
+def _check_k(k: int) -> None:
+    if k % 32 != 0:
+        raise RuntimeError(f"the last dimension must be divisible by 32, the size of a block (got {k})")
+
+
+def _new_quantized(lead, R: int, K: int, fmt: int, want_rows: bool, want_tc: bool, device):
+    if not want_rows and not want_tc:
+        raise RuntimeError("ask for at least one layout of the scales (want_rows, want_tc)")
+    codes = (torch.empty((*lead, K // 2), dtype=torch.uint8, device=device) if fmt == L.MXFP4
+             else torch.empty((*lead, K), dtype=torch.float8_e4m3fn, device=device))
+    scales = torch.empty((*lead, K // 32), dtype=torch.uint8, device=device) if want_rows else None
+    tc = torch.empty((mx_scales_numel(R, K),), dtype=torch.uint8, device=device) if want_tc else None
+    return codes, scales, tc
+
+
+def _codes_of(codes: torch.Tensor) -> Tuple[int, int, int]:
+    """(format, R, K) of a codes tensor"""
+    R, width = _rows_of(codes)
+    if codes.dtype == torch.uint8:
+        K, fmt = 2 * width, L.MXFP4
+    elif codes.dtype == torch.float8_e4m3fn:
+        K, fmt = width, L.MXFP8
+    else:
+        raise RuntimeError(f"Invalid datatype {codes.dtype} of codes (uint8 for mxfp4, float8_e4m3fn for mxfp8)")
+    _check_k(K)
+    return fmt, R, K
+
+
+def _check_scales(scales: torch.Tensor, layout: str, R: int, K: int) -> None:
+    """the kernels read whole records, and every row: a short buffer would be read past its end"""
+    if layout not in _SCALES:
+        raise ValueError(f"unknown scale layout {layout!r} (have 'rows' and 'tc')")
+    need = R * (K // 32) if layout == "rows" else mx_scales_numel(R, K)
+    if scales.dtype not in _SCALE_TYPES or scales.numel() != need or not scales.is_contiguous():
+        raise RuntimeError(f"{layout!r} scales of a ({R}, {K}) matrix are {need} contiguous bytes (uint8), got {scales.numel()} of "
+                           f"{scales.dtype}")
+
+
+def mx_quantize(x: torch.Tensor, fmt: str = "mxfp4", want_rows: bool = True, want_tc: bool = False):
+    """Quantise x (..., K), float16 / bfloat16 / float32, along its last dimension in one pass.
+
+    Returns (codes, scales (..., K / 32) or None, tensor-core-order scales or None).
+    """
+    f = _check_fmt(fmt)
+    R, K = _rows_of(x)
+    if x.dtype not in _DT:
+        raise RuntimeError(f"Invalid datatype {x.dtype} of dense matrix")
+    _check_k(K)
+    _require_cuda(x)
+    codes, scales, tc = _new_quantized(x.shape[:-1], R, K, f, want_rows, want_tc, x.device)
+    if R * K:
+        m, ld = _matrix(x, R, 16)
+        with _on_device(x):
+            L.check(L.lib().s24_mx_quantize(_p(m), R, K, ld, _DT[x.dtype], f, _p(codes), _p(scales), _p(tc), _stream(x)))
+    return codes, scales, tc
+
+
+def mx_dequantize(codes: torch.Tensor, scales: torch.Tensor, layout: str = "rows", dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """Read (codes, scales) back as a (..., K) tensor of `dtype` (float16, bfloat16 or float32), rounded once."""
+    f, R, K = _codes_of(codes)
+    if dtype not in _DT:
+        raise RuntimeError(f"Invalid datatype {dtype} of dense matrix")
+    _check_scales(scales, layout, R, K)
+    _require_cuda(codes, scales)
+    out = torch.empty((*codes.shape[:-1], K), dtype=dtype, device=codes.device)
+    if R * K:
+        c = codes if codes.is_contiguous() and codes.data_ptr() % 16 == 0 else codes.clone(memory_format=torch.contiguous_format)
+        with _on_device(codes):
+            L.check(L.lib().s24_mx_dequantize(_p(c), _p(scales), _SCALES[layout], _p(out), R, K, f, _DT[dtype], _stream(codes)))
+    return out
+
+
+def mx_scales_convert(scales: torch.Tensor, from_layout: str, to_layout: str, R: int, K: int) -> torch.Tensor:
+    """Re-lay the scales of an (R, K) matrix between "rows" ((R, K / 32)) and "tc"."""
+    _check_k(K)
+    _check_scales(scales, from_layout, R, K)
+    if to_layout not in _SCALES or to_layout == from_layout:
+        raise ValueError(f"cannot convert scales from {from_layout!r} to {to_layout!r}")
+    _require_cuda(scales)
+    shape = (R, K // 32) if to_layout == "rows" else (mx_scales_numel(R, K),)
+    out = torch.empty(shape, dtype=torch.uint8, device=scales.device)
+    if R * K:
+        with _on_device(scales):
+            L.check(L.lib().s24_mx_scales_convert(_p(scales), _SCALES[from_layout], _p(out), _SCALES[to_layout], R, K, _stream(scales)))
+    return out
+
+
+def mx_rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: Optional[torch.Tensor] = None, fmt: str = "mxfp8",
+                want_rows: bool = True, want_tc: bool = False):
+    """Root-mean-square norm over the last dimension with the residual's addition, quantised as it is computed:
+    h = x + residual (rounded to x's type; x itself without a residual), y = h * weight / sqrt(mean(h^2) + eps).
+
+    x and residual (..., K) and weight (K) share a type, float16 or bfloat16; K is at most 65536.  y is not rounded
+    before it is quantised.  Returns (codes, scales or None, tensor-core-order scales or None, h).
+    """
+    f = _check_fmt(fmt)
+    R, K = _rows_of(x)
+    if x.dtype not in (torch.float16, torch.bfloat16):
+        raise RuntimeError(f"Invalid datatype {x.dtype} of dense matrix")
+    _check_k(K)
+    if weight.dtype != x.dtype or tuple(weight.shape) != (K,):
+        raise RuntimeError(f"`weight` must be a ({K},) {x.dtype} tensor, got {tuple(weight.shape)} {weight.dtype}")
+    if residual is not None and (residual.dtype != x.dtype or residual.shape != x.shape):
+        raise RuntimeError(f"`residual` must be a {tuple(x.shape)} {x.dtype} tensor, got {tuple(residual.shape)} {residual.dtype}")
+    if K > L.MX_NORM_MAX_K:
+        raise RuntimeError(f"rows of at most {L.MX_NORM_MAX_K} elements (got {K})")
+    _require_cuda(x, weight, residual)
+    codes, scales, tc = _new_quantized(x.shape[:-1], R, K, f, want_rows, want_tc, x.device)
+    h = x if residual is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if R * K:
+        m, ldx = _matrix(x, R, 16)
+        r, ldr = (None, 0) if residual is None else _matrix(residual, R, 16)
+        w, _ = _matrix(weight, 1, 16)
+        with _on_device(x):
+            L.check(L.lib().s24_mx_rms_norm(_p(m), _p(r), _p(w), _p(None if residual is None else h), R, K, ldx, ldr, float(eps),
+                                            _DT[x.dtype], f, _p(codes), _p(scales), _p(tc), _stream(x)))
+    return codes, scales, tc, h
+
+
+def mx_matmul(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_scales: torch.Tensor, out_dtype: torch.dtype = torch.bfloat16,
+              out: Optional[torch.Tensor] = None, manual_config: Optional[dict] = None) -> torch.Tensor:
+    """C (..., N) = deq(a) (..., K) @ deq(b) (N, K)^T with fp32 accumulation, rounded once to `out_dtype`.
+
+    a and b are codes of either format, their scales in tensor-core order (`want_tc=True`, or mx_scales_convert);
+    K must be a multiple of 128 where the formats differ.  `out` (2-dimensional, of `out_dtype`) must not
+    overlap the operands.
+    """
+    fa, M, K = _codes_of(a)
+    fb, N, Kb = _codes_of(b)
+    if b.dim() != 2:
+        raise RuntimeError(f"b must be 2-dimensional (N, K), got {b.dim()} dimensions")
+    if K != Kb or K == 0:
+        raise RuntimeError(f"a has {K} elements a row and b {Kb}: they must be equal and not 0")
+    if fa != fb and K % 128 != 0:
+        raise RuntimeError(f"operands of different formats need K % 128 == 0 (got {K})")
+    if out_dtype not in _DT:
+        raise RuntimeError(f"Invalid datatype {out_dtype} of the product")
+    _check_scales(a_scales, "tc", M, K)
+    _check_scales(b_scales, "tc", N, K)
+    _require_cuda(a, a_scales, b, b_scales, out)
+    if out is None:
+        c = torch.empty((*a.shape[:-1], N), dtype=out_dtype, device=a.device)
+        ldc = N
+    else:
+        c = out
+        ldc = c.stride(0) if c.dim() == 2 and M > 1 else N
+        if tuple(c.shape) != (M, N) or c.dtype != out_dtype or (N > 1 and c.stride(1) != 1) or ldc < N:
+            raise RuntimeError(f"`out` must be a ({M}, {N}) {out_dtype} tensor with unit column stride and rows that do not overlap")
+    if M * N:
+        ma, lda = _matrix(a, M, 32 if fa == L.MXFP4 != fb else 16)
+        mb, ldb = _matrix(b, N, 32 if fb == L.MXFP4 != fa else 16)
+        with _on_device(a):
+            L.check(L.lib().s24_mx_matmul(_p(ma), _p(a_scales), _p(mb), _p(b_scales), _p(c), M, N, K, lda, ldb, ldc, fa, fb, _DT[out_dtype],
+                                          _tile_cfg(manual_config), _stream(a)))
+            _after_gemm(a)
+    return c

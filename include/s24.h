@@ -53,6 +53,23 @@
  *                     point that writes this layout sets the filler itself, with an
  *                     asynchronous memset on the caller's stream before its kernel; a caller
  *                     that builds such a buffer on its own must do the same.
+ *
+ * Microscaled formats (s24_mx_*): the library's other compression, by number format.  Every block of
+ * 32 consecutive elements of a row shares a power of two and each element is a 4-bit (e2m1, largest
+ * value 6, emax 2) or 8-bit (e4m3, largest 448, emax 8) float.  With a = max |v_i| over a block
+ *   scale  s = clamp(floor(log2 a) - emax + 127, 0, 254), s = 0 for a = 0: one byte,
+ *   codes  v * 2^(127 - s) rounded to the element type, half to even, saturating,
+ * and the block reads back as element * 2^(s - 127).  A block with a NaN or an infinity has s = 255
+ * and codes 0 and reads back as NaN.  S24_MXFP4 codes are (R, K/2) bytes, element 2i in the low half
+ * of byte i; S24_MXFP8 codes are (R, K) bytes.  Scale layouts:
+ *   S24_SCALES_ROWS   scales[r][k / 32], (R, K/32) bytes
+ *   S24_SCALES_TC     records of 512 bytes per (128-row tile t, 128-column chunk c), ordered [t][c];
+ *                     the scale of row r, block b = k / 32 is byte
+ *                     ((r/128) * ceil(K/128) + b/4) * 512 + (r%32)*16 + (r%128)/32*4 + b%4.
+ *                     This is the image tcgen05.cp moves into tensor memory for the block-scaled
+ *                     products.  Positions outside the matrix hold 0 (a finite scale; the codes
+ *                     they meet read as zero); every entry point that writes this layout writes
+ *                     them, and a caller that builds such a buffer on its own must do the same.
  */
 #ifndef S24_H_
 #define S24_H_
@@ -83,7 +100,7 @@ extern "C" {
 /* element types */
 #define S24_FP16 0
 #define S24_BF16 1
-/* accepted by s24_compress_other only */
+/* accepted by s24_compress_other (all three) and the s24_mx_* calls that say so (S24_FP32) */
 #define S24_INT8 2
 #define S24_INT32 3
 #define S24_FP32 4
@@ -104,6 +121,12 @@ extern "C" {
 #define S24_META_LOGICAL 0
 #define S24_META_REF 1
 #define S24_META_TC 2
+
+/* microscaled formats and the layouts of their scales */
+#define S24_MXFP4 0
+#define S24_MXFP8 1
+#define S24_SCALES_ROWS 0
+#define S24_SCALES_TC 1
 
 /* Optional tile choice for the GEMM entry points; NULL or zeros = heuristic.
  * Mirrors the keys of the reference's manual_config (gluon_ws_sparse.py:629-636). */
@@ -276,6 +299,54 @@ S24_API int s24_spmm_prune_out(const void* vals, const void* meta_tc, const void
 S24_API int s24_spmm_prune_in(const void* A, int64_t lda, const void* B, void* C,
                       int64_t M, int64_t N, int64_t K, int64_t ldb, int64_t ldc,
                       int dtype, int mode, int tie, void* stream);
+
+/* bytes of a S24_SCALES_TC buffer of an (R, K) matrix: ceil(R/128) * ceil(K/128) * 512; 0 if R or K is not positive */
+S24_API size_t s24_mx_scales_tc_bytes(int64_t R, int64_t K);
+
+/*
+ * Quantise x (R, K; row stride ld elements; S24_FP16, S24_BF16 or S24_FP32) to `fmt` in one pass: codes
+ * (contiguous) and the scales in either layout or both (one of the two pointers may be NULL).
+ * K % 32 == 0, row stride a multiple of 16 bytes; x, codes and scales_tc 16-byte aligned.  R = 0 or
+ * K = 0 does nothing.
+ */
+S24_API int s24_mx_quantize(const void* x, int64_t R, int64_t K, int64_t ld, int dtype, int fmt,
+                    void* codes, void* scales, void* scales_tc, void* stream);
+
+/* Read codes and scales (in `layout`) back: out (R, K) contiguous, S24_FP16, S24_BF16 or S24_FP32, rounded once.
+ * codes and out 16-byte aligned, K % 32 == 0. */
+S24_API int s24_mx_dequantize(const void* codes, const void* scales, int layout, void* out, int64_t R, int64_t K,
+                      int fmt, int dtype, void* stream);
+
+/* Re-lay the scales of an (R, K) matrix between the two layouts; src and dst must not overlap. */
+S24_API int s24_mx_scales_convert(const void* src, int from_layout, void* dst, int to_layout, int64_t R, int64_t K, void* stream);
+
+/*
+ * Root-mean-square norm with the residual's addition, quantised as it is computed:
+ *   h = round(x + residual), y = h * weight / sqrt(mean(h^2) + eps), (codes, scales) = quantise(y).
+ * h (R, K contiguous, x's type) is written only with a residual and may be the residual itself; without
+ * one (NULL) h = x and the pointer is ignored.  y is not rounded before the quantisation: codes and
+ * scales are those of the formula in 64 bits (values of y beyond the fp32 range count as infinite).
+ * x and residual have row strides ldx, ldr (elements, multiples of 8); weight is (K) of x's type
+ * (S24_FP16 or S24_BF16).  K % 32 == 0, K <= S24_MX_NORM_MAX_K, eps in [1e-30, 1e30], 16-byte aligned
+ * pointers (scales excepted), either scale pointer may be NULL.
+ */
+#define S24_MX_NORM_MAX_K 65536
+S24_API int s24_mx_rms_norm(const void* x, const void* residual, const void* weight, void* h, int64_t R, int64_t K,
+                    int64_t ldx, int64_t ldr, double eps, int dtype, int fmt,
+                    void* codes, void* scales, void* scales_tc, void* stream);
+
+/*
+ * C (M, N) = A . B^T of two quantised matrices, A (M, K) and B (N, K) (activations (tokens, hidden) and a
+ * weight (out, in), say), fp32 accumulation, C in S24_FP16, S24_BF16 or S24_FP32 with row stride ldc
+ * elements.  Each operand is S24_MXFP4 or S24_MXFP8, with its row stride in bytes and its scales in
+ * S24_SCALES_TC order.  K % 32 == 0, and K % 128 == 0 where the formats differ; any M and N.  Codes:
+ * rows and pointers on 16 bytes, a S24_MXFP4 operand beside a S24_MXFP8 one on 32; scales on 16; C on its
+ * element.  Two operands of 4 bits run at twice the rate of the other pairs.  cfg as for s24_spmm, with
+ * the tiles that call names in its error message.
+ */
+S24_API int s24_mx_matmul(const void* a, const void* a_scales, const void* b, const void* b_scales, void* C,
+                  int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb, int64_t ldc,
+                  int fmt_a, int fmt_b, int out_dtype, const s24_tile_cfg* cfg, void* stream);
 
 /*
  * Multi-GPU: replicated result without a separate all-gather (the reference is single-GPU; no
