@@ -103,6 +103,9 @@ struct MxParams {
     unsigned long long wait_limit_ns;
 };
 
+constexpr int kStorePitch = 17;                              // words: 16 of a row and one against bank conflicts
+constexpr int kStoreWarpBytes = 32 * kStorePitch * 4;
+
 template <int G, int BN, bool F4, int ST>
 struct MxCfg {
     static constexpr int kG = G;
@@ -118,44 +121,72 @@ struct MxCfg {
     static constexpr int kSABytes = kChunks * mx::kRecordBytes;
     static constexpr int kSBBytes = kTilesB * kChunks * mx::kRecordBytes;
     static constexpr int kStageBytes = kABytes + kBBytes + kSABytes + kSBBytes;
-    static constexpr int kAcc = BN >= 256 ? 1 : 2;
-    static constexpr int kScaleCol0 = kAcc * BN;
+    static constexpr int kAccStep = BN >= 256 ? 224 : BN;       // first column of the second accumulator
+    static constexpr int kScaleCol0 = kAccStep + BN;
     static constexpr int kScaleCols = 4 * kChunks * (1 + kTilesB);
-    static constexpr int kSmemBytes = ST * kStageBytes + 1024 + 256;
-    static_assert(kScaleCol0 + ST * kScaleCols <= (int)kTmemCols, "tensor memory budget");
+    static constexpr int kStoreBytes = 8 * kStoreWarpBytes;
+    static constexpr int kSmemBytes = ST * kStageBytes + kStoreBytes + 1024 + 256;
+    static_assert(kScaleCol0 + kScaleCols <= (int)kTmemCols, "tensor memory budget");
     static_assert(kSmemBytes <= 232448, "shared memory budget");
-    static_assert(8 * (2 * ST + 2 * kAcc) + 16 <= 256, "barrier block");
+    static_assert(8 * (2 * ST + 2) + 16 <= 256, "barrier block");
 };
 
-// one row's 32 accumulator columns to memory
-__device__ __forceinline__ void mx_store32(const MxParams& p, int row, int col, const uint32_t* r)
+// 32 rows (one per lane) x 32 accumulator columns to C.  Rows that allow 16-byte stores take them straight from
+// the registers (64 or 128 bytes per lane); others go through 2 KB of shared memory, so that 16 lanes write one
+// row's 64 bytes instead of every lane its own row in elements.
+__device__ __forceinline__ void mx_store32(const MxParams& p, int row0, int col, const uint32_t (&r)[32], uint32_t staging, int lane)
 {
-    if (row >= p.M || col >= p.N) return;
-    const int64_t at = (int64_t)row * p.ldc + col;
-    const bool whole = p.wide && col + 32 <= p.N;
-    if (p.out == S24_FP32) {
-        float* c = static_cast<float*>(p.C) + at;
-        if (whole) {
+    if (row0 >= p.M || col >= p.N) return;   // the same for the whole warp
+    const bool f32 = p.out == S24_FP32;
+    uint32_t q[32];
+    if (f32) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) reinterpret_cast<uint4*>(c)[i] = make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
-        } else {
+        for (int i = 0; i < 32; ++i) q[i] = r[i];
+    } else {
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-                if (col + i < p.N) c[i] = __uint_as_float(r[i]);
+        for (int i = 0; i < 16; ++i) q[i] = pack2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]), p.out == S24_BF16);
+    }
+    if (p.wide && col + 32 <= p.N) {
+        const int64_t at = (int64_t)(row0 + lane) * p.ldc + col;
+        if (row0 + lane < p.M) {
+            uint4* c = reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.C) + at * (f32 ? 4 : 2));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) c[i] = make_uint4(q[4 * i], q[4 * i + 1], q[4 * i + 2], q[4 * i + 3]);
+            if (f32) {
+#pragma unroll
+                for (int i = 4; i < 8; ++i) c[i] = make_uint4(q[4 * i], q[4 * i + 1], q[4 * i + 2], q[4 * i + 3]);
+            }
         }
         return;
     }
-    uint16_t* c = static_cast<uint16_t*>(p.C) + at;
-    uint32_t q[16];
+    const int word = lane & 15;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) q[i] = pack2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]), p.out == S24_BF16);
-    if (whole) {
+    for (int part = 0; part < 2; ++part) {
+        if (part == 1 && !f32) break;
+        __syncwarp();
 #pragma unroll
-        for (int i = 0; i < 4; ++i) reinterpret_cast<uint4*>(c)[i] = make_uint4(q[4 * i], q[4 * i + 1], q[4 * i + 2], q[4 * i + 3]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 32; ++i)
-            if (col + i < p.N) c[i] = (uint16_t)(q[i >> 1] >> (16 * (i & 1)));
+        for (int i = 0; i < 16; ++i) st_shared_u32(staging + (uint32_t)(lane * kStorePitch + i) * 4, q[16 * part + i]);
+        __syncwarp();
+#pragma unroll 4
+        for (int i = 0; i < 16; ++i) {
+            const int rr = 2 * i + (lane >> 4), row = row0 + rr;
+            uint32_t v;
+            asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(staging + (uint32_t)(rr * kStorePitch + word) * 4) : "memory");
+            if (row >= p.M) continue;
+            if (f32) {
+                const int c = col + 16 * part + word;
+                if (c < p.N) static_cast<float*>(p.C)[(int64_t)row * p.ldc + c] = __uint_as_float(v);
+            } else {
+                const int c = col + 2 * word;
+                uint16_t* dst = static_cast<uint16_t*>(p.C) + (int64_t)row * p.ldc + c;
+                if (c + 1 < p.N && (reinterpret_cast<uintptr_t>(dst) & 3u) == 0) {
+                    *reinterpret_cast<uint32_t*>(dst) = v;
+                } else {
+                    if (c < p.N) dst[0] = (uint16_t)v;
+                    if (c + 1 < p.N) dst[1] = (uint16_t)(v >> 16);
+                }
+            }
+        }
     }
 }
 
@@ -164,7 +195,7 @@ __global__ void __launch_bounds__(kMxThreads, 1)
 mx_matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
                  const __grid_constant__ CUtensorMap tm_sa, const __grid_constant__ CUtensorMap tm_sb, const MxParams p)
 {
-    constexpr int G = Cfg::kG, BN = Cfg::kBN, ST = Cfg::kStages, ACC = Cfg::kAcc;
+    constexpr int G = Cfg::kG, BN = Cfg::kBN, ST = Cfg::kStages;
 
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -172,12 +203,12 @@ mx_matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
     const uint32_t smem_b = smem_a + ST * Cfg::kABytes;
     const uint32_t smem_sa = smem_b + ST * Cfg::kBBytes;
     const uint32_t smem_sb = smem_sa + ST * Cfg::kSABytes;
-    const uint32_t bars = smem_sb + ST * Cfg::kSBBytes;
-    const uint32_t bar_full = bars;
+    const uint32_t smem_store = smem_sb + ST * Cfg::kSBBytes;
+    const uint32_t bar_full = smem_store + Cfg::kStoreBytes;
     const uint32_t bar_empty = bar_full + 8 * ST;
     const uint32_t bar_acc_full = bar_empty + 8 * ST;
-    const uint32_t bar_acc_empty = bar_acc_full + 8 * ACC;
-    const uint32_t tmem_slot = bar_acc_empty + 8 * ACC;
+    const uint32_t bar_acc_empty = bar_acc_full + 8;
+    const uint32_t tmem_slot = bar_acc_empty + 8;
     const uint32_t abort_addr = tmem_slot + 8;
     uint8_t* smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
     volatile uint32_t* tmem_slot_ptr = reinterpret_cast<volatile uint32_t*>(smem_gen + (tmem_slot - smem_base));
@@ -200,10 +231,8 @@ mx_matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
             mbar_init(bar_full + 8 * s, 1);   // one arrive (the leader's producer) + both CTAs' bytes
             mbar_init(bar_empty + 8 * s, 1);
         }
-        for (int a = 0; a < ACC; ++a) {
-            mbar_init(bar_acc_full + 8 * a, 1);
-            mbar_init(bar_acc_empty + 8 * a, 8 * G);
-        }
+        mbar_init(bar_acc_full, 1);
+        mbar_init(bar_acc_empty, 8 * G);   // the epilogue warps of every CTA
         *abort_flag = 0;
         fence_barrier_init();
     }
@@ -256,16 +285,20 @@ mx_matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
         // ------------------------------------------------------------ MMA issuer (leader CTA only)
         if (leader && elect_one()) {
             const uint32_t idesc = make_idesc_scaled(p.a_format, p.b_format, 128 * G, BN);
-            int s = 0, a = 0;
-            uint32_t ph = 0, acc_phase = 0;
+            const uint32_t sfa = tmem_base + (uint32_t)Cfg::kScaleCol0;
+            const uint32_t sfb = sfa + 4 * Cfg::kChunks;
+            int s = 0, n = 0;   // n: tiles done
+            uint32_t ph = 0;
             bool ok = true;
-            for (int t = unit; t < num_tiles && ok && !*abort_flag; t += num_units) {
-                if (!mbar_wait(bar_acc_empty + 8 * a, acc_phase ^ 1u, p.wait_limit_ns)) {
+            for (int t = unit; t < num_tiles && ok && !*abort_flag; t += num_units, ++n) {
+                // the epilogue has read what the previous tile's accumulator shares with this one's (and, before it, all
+                // of the tile before that, which had this accumulator)
+                if (n > 0 && !mbar_wait(bar_acc_empty, (uint32_t)(n - 1) & 1u, p.wait_limit_ns)) {
                     report_timeout(p.status, abort_flag, 3);
                     break;
                 }
                 tc_fence_after();
-                const uint32_t tmem_d = tmem_base + (uint32_t)(a * BN);
+                const uint32_t tmem_d = tmem_base + (uint32_t)((n & 1) * Cfg::kAccStep);
                 for (int kt = 0; kt < ktiles; ++kt) {
                     if (!mbar_wait(bar_full + 8 * s, ph, p.wait_limit_ns)) {
                         report_timeout(p.status, abort_flag, 2);
@@ -273,8 +306,7 @@ mx_matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
                         break;
                     }
                     tc_fence_after();
-                    const uint32_t sfa = tmem_base + (uint32_t)(Cfg::kScaleCol0 + s * Cfg::kScaleCols);
-                    const uint32_t sfb = sfa + 4 * Cfg::kChunks;
+                    // tcgen05.cp and tcgen05.mma run in the order of issue, so one set of scale columns does
 #pragma unroll
                     for (int c = 0; c < Cfg::kChunks; ++c) {
                         tc_cp_scales<G>(sfa + 4 * c, make_smem_desc(smem_sa + s * Cfg::kSABytes + c * mx::kRecordBytes, 128, 128, kSwizzleNone));
@@ -297,9 +329,8 @@ mx_matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
                     if (++s == ST) { s = 0; ph ^= 1u; }
                 }
                 if (!ok) break;
-                if (G == 2) tc_commit_pair(bar_acc_full + 8 * a, 3);
-                else tc_commit<1>(bar_acc_full + 8 * a);
-                if (++a == ACC) { a = 0; acc_phase ^= 1u; }
+                if (G == 2) tc_commit_pair(bar_acc_full, 3);
+                else tc_commit<1>(bar_acc_full);
             }
         }
     } else {
@@ -307,34 +338,43 @@ mx_matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
         const int quad = warp & 3;
         const int half = (warp - 2) >> 2;
         constexpr int CW = BN / 2;
-        int a = 0;
-        uint32_t acc_phase = 0;
+        const uint32_t staging = smem_store + (uint32_t)(warp - 2) * kStoreWarpBytes;
         const uint32_t acc_empty = (G == 2) ? mapa(bar_acc_empty, 0) : bar_acc_empty;
-        for (int t = unit; t < num_tiles && !*abort_flag; t += num_units) {
+        int n = 0;
+        for (int t = unit; t < num_tiles && !*abort_flag; t += num_units, ++n) {
             int tm, tn;
             tile_coords(t, num_m, num_n, tm, tn);
-            if (!__all_sync(0xFFFFFFFFu, mbar_wait(bar_acc_full + 8 * a, acc_phase, p.wait_limit_ns))) {
+            if (!__all_sync(0xFFFFFFFFu, mbar_wait(bar_acc_full, (uint32_t)n & 1u, p.wait_limit_ns))) {
                 if (lane == 0) report_timeout(p.status, abort_flag, 4);
                 break;
             }
             tc_fence_after();
-            const uint32_t tacc = tmem_base + (uint32_t)(a * BN + half * CW) + ((uint32_t)(32 * quad) << 16);
-            const int row = (tm * G + (int)cta_rank) * 128 + 32 * quad + lane;
+            const uint32_t tacc = tmem_base + (uint32_t)((n & 1) * Cfg::kAccStep + half * CW) + ((uint32_t)(32 * quad) << 16);
+            const int row0 = (tm * G + (int)cta_rank) * 128 + 32 * quad;
             const int col = tn * BN + half * CW;
+            // The 32 columns that both accumulators cover are the first's last ones and the second's first ones: the warp
+            // that owns them reads them first and hands them back; every warp arrives, whether it has a share or not.
+            const int first = (n & 1) ? 0 : CW - 32;
+            const bool shares = half == ((n & 1) ? 0 : 1);
+            if (!shares) {
+                tc_fence_before();   // its reads of the tile before
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(acc_empty);
+            }
 #pragma unroll 1
-            for (int c = 0; c < CW; c += 32) {
+            for (int i = 0; i < CW / 32; ++i) {
+                const int c = i == 0 ? first : (n & 1) ? 32 * i : 32 * (i - 1);
                 uint32_t r[32];
                 tc_ld_32x32b_x32(tacc + (uint32_t)c, r);
                 tc_wait_ld();
-                if (c + 32 == CW) {
+                if (shares && i == 0) {
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive_cluster(acc_empty + 8 * a);
+                    if (lane == 0) mbar_arrive_cluster(acc_empty);
                 }
-                mx_store32(p, row, col + c, r);
+                mx_store32(p, row0, col + c, r, staging, lane);
                 __syncwarp();
             }
-            if (++a == ACC) { a = 0; acc_phase ^= 1u; }
         }
     }
 
@@ -346,6 +386,211 @@ mx_matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
     if (warp == 1) {
         tc_fence_after();
         tmem_dealloc<G>(tmem_base, kTmemCols);
+    }
+}
+
+// ---------------------------------------------------------------- few rows
+//
+// With few rows on one side (a decoding step) the product is the reading of the other side's codes.  That side
+// ("long") takes the 128 rows of the MMA, the few rows its NT columns, and K is split over the S CTAs of a cluster so
+// that all SMs read: each CTA multiplies its share of the k-tiles, leaves its partial sums (fp32) in its shared
+// memory, and each then adds 1 / S of the columns over the S CTAs, in the order of their ranks, and stores them.
+// No workspace, no atomics, one launch, the same sums whatever order the CTAs run in.
+
+struct FewParams {
+    void* C;
+    int64_t stride_long, stride_few;   // elements of C between rows of the long side, and of the few
+    int n_long, n_few, ktiles;
+    int out;
+    uint32_t a_format, b_format;       // of the long side, and of the few
+    uint32_t tx_bytes;
+    int* status;
+    unsigned long long wait_limit_ns;
+};
+
+constexpr int kFewThreads = 192;   // producer, MMA issuer, four epilogue warps
+
+template <bool F4, int NT, int ST>
+struct FewCfg {
+    static constexpr bool kF4 = F4;
+    static constexpr int kNT = NT;
+    static constexpr int kStages = ST;
+    static constexpr int kChunks = F4 ? 2 : 1;
+    static constexpr int kABytes = 128 * 128;
+    static constexpr int kBBytes = NT * 128;
+    static constexpr int kSBytes = kChunks * mx::kRecordBytes;
+    static constexpr int kStageBytes = kABytes + kBBytes + 2 * kSBytes;
+    static constexpr int kScaleCols = 8 * kChunks;
+    static constexpr int kScaleCol0 = NT;
+    static constexpr int kTmem = NT + kScaleCols <= 32 ? 32 : NT + kScaleCols <= 64 ? 64 : NT + kScaleCols <= 128 ? 128 : 256;
+    static constexpr int kSmemBytes = ST * kStageBytes + 1024 + 128;
+    static_assert(ST * kStageBytes >= NT * 128 * 4, "the partial sums take the place of the stages");
+    static_assert(8 * (2 * ST + 1) + 16 <= 128, "barrier block");
+    static_assert(2 * (kSmemBytes + 1024) <= 233472, "two CTAs per SM");
+};
+
+__device__ __forceinline__ float ld_cluster_f32(uint32_t cluster_addr)
+{
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr) : "memory");
+    return v;
+}
+
+__device__ __forceinline__ void few_store(const FewParams& p, int i, int j, float v)
+{
+    if (i >= p.n_long || j >= p.n_few) return;
+    const int64_t at = (int64_t)i * p.stride_long + (int64_t)j * p.stride_few;
+    if (p.out == S24_FP32) static_cast<float*>(p.C)[at] = v;
+    else if (p.out == S24_BF16) static_cast<__nv_bfloat16*>(p.C)[at] = __float2bfloat16_rn(v);
+    else static_cast<__half*>(p.C)[at] = __float2half_rn(v);
+}
+
+template <class Cfg>
+__global__ void __launch_bounds__(kFewThreads)
+mx_matmul_few_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
+                     const __grid_constant__ CUtensorMap tm_sa, const __grid_constant__ CUtensorMap tm_sb, const FewParams p)
+{
+    constexpr int ST = Cfg::kStages, NT = Cfg::kNT;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    const uint32_t smem_a = smem_base;
+    const uint32_t smem_b = smem_a + ST * Cfg::kABytes;
+    const uint32_t smem_sa = smem_b + ST * Cfg::kBBytes;
+    const uint32_t smem_sb = smem_sa + ST * Cfg::kSBytes;
+    const uint32_t bar_full = smem_sb + ST * Cfg::kSBytes;
+    const uint32_t bar_empty = bar_full + 8 * ST;
+    const uint32_t bar_acc = bar_empty + 8 * ST;
+    const uint32_t tmem_slot = bar_acc + 8;
+    const uint32_t abort_addr = tmem_slot + 8;
+    uint8_t* smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
+    volatile uint32_t* tmem_slot_ptr = reinterpret_cast<volatile uint32_t*>(smem_gen + (tmem_slot - smem_base));
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(smem_gen + (abort_addr - smem_base));
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int split = (int)gridDim.x;                 // the cluster spans the grid's x
+    const int rank = (int)blockIdx.x;
+    const int row0 = (int)blockIdx.y * 128;
+    const int kt0 = (int)((int64_t)p.ktiles * rank / split), kt1 = (int)((int64_t)p.ktiles * (rank + 1) / split);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < ST; ++s) {
+            mbar_init(bar_full + 8 * s, 1);
+            mbar_init(bar_empty + 8 * s, 1);
+        }
+        mbar_init(bar_acc, 1);
+        *abort_flag = 0;
+        fence_barrier_init();
+    }
+    if (warp == 0 && lane == 0) {
+        prefetch_tensormap(&tm_a);
+        prefetch_tensormap(&tm_b);
+        prefetch_tensormap(&tm_sa);
+        prefetch_tensormap(&tm_sb);
+    }
+    if (warp == 1) {
+        tmem_alloc<1>(tmem_slot, Cfg::kTmem);
+        tmem_relinquish<1>();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot_ptr;
+
+    if (warp == 0) {
+        if (elect_one()) {
+            int s = 0;
+            uint32_t ph = 0;
+            for (int kt = kt0; kt < kt1; ++kt) {
+                if (!mbar_wait(bar_empty + 8 * s, ph ^ 1u, p.wait_limit_ns)) {
+                    report_timeout(p.status, abort_flag, 1);
+                    break;
+                }
+                const uint32_t full = bar_full + 8 * s;
+                mbar_arrive_expect_tx(full, p.tx_bytes);
+                tma_load_2d(smem_a + s * Cfg::kABytes, &tm_a, kt * 128, row0, full);
+                tma_load_3d<1>(smem_sa + s * Cfg::kSBytes, &tm_sa, 0, kt * Cfg::kChunks, row0 / 128, full);
+                tma_load_2d(smem_b + s * Cfg::kBBytes, &tm_b, kt * 128, 0, full);
+                tma_load_3d<1>(smem_sb + s * Cfg::kSBytes, &tm_sb, 0, kt * Cfg::kChunks, 0, full);
+                if (++s == ST) { s = 0; ph ^= 1u; }
+            }
+        }
+    } else if (warp == 1) {
+        if (elect_one()) {
+            const uint32_t idesc = make_idesc_scaled(p.a_format, p.b_format, 128, NT);
+            const uint32_t sfa = tmem_base + (uint32_t)Cfg::kScaleCol0, sfb = sfa + 4 * Cfg::kChunks;
+            int s = 0;
+            uint32_t ph = 0;
+            bool ok = true;
+            for (int kt = kt0; kt < kt1; ++kt) {
+                if (!mbar_wait(bar_full + 8 * s, ph, p.wait_limit_ns)) {
+                    report_timeout(p.status, abort_flag, 2);
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+#pragma unroll
+                for (int c = 0; c < Cfg::kChunks; ++c) {
+                    tc_cp_scales<1>(sfa + 4 * c, make_smem_desc(smem_sa + s * Cfg::kSBytes + c * mx::kRecordBytes, 128, 128, kSwizzleNone));
+                    tc_cp_scales<1>(sfb + 4 * c, make_smem_desc(smem_sb + s * Cfg::kSBytes + c * mx::kRecordBytes, 128, 128, kSwizzleNone));
+                }
+                const uint64_t adesc = make_smem_desc(smem_a + s * Cfg::kABytes, 16, 1024, kSwizzle128B);
+                const uint64_t bdesc = make_smem_desc(smem_b + s * Cfg::kBBytes, 16, 1024, kSwizzle128B);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t c = Cfg::kF4 ? j >> 1 : 0, id = Cfg::kF4 ? (j & 1) * 2 : j;
+                    tc_mma_scaled<1, Cfg::kF4>(tmem_base, adesc + (uint64_t)(j * 2), bdesc + (uint64_t)(j * 2), idesc | (id << 4) | (id << 29), sfa + 4 * c,
+                                               sfb + 4 * c, (kt != kt0 || j != 0) ? 1u : 0u);
+                }
+                tc_commit<1>(bar_empty + 8 * s);
+                if (++s == ST) { s = 0; ph ^= 1u; }
+            }
+            if (ok) tc_commit<1>(bar_acc);
+        }
+    } else {
+        const int quad = warp & 3;
+        const int row = 32 * quad + lane;
+        if (__all_sync(0xFFFFFFFFu, mbar_wait(bar_acc, 0, p.wait_limit_ns))) {
+            tc_fence_after();
+            const uint32_t tacc = tmem_base + ((uint32_t)(32 * quad) << 16);
+#pragma unroll
+            for (int c = 0; c < NT; c += 16) {
+                if (c >= p.n_few) break;
+                uint32_t r[16];
+                tc_ld_32x32b_x16(tacc + (uint32_t)c, r);
+                tc_wait_ld();
+                if (split == 1) {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) few_store(p, row0 + row, c + j, __uint_as_float(r[j]));
+                } else {   // every copy into the stages and every MMA that reads them is done
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) st_shared_u32(smem_base + (uint32_t)((c + j) * 128 + row) * 4, r[j]);
+                }
+            }
+        } else if (lane == 0) {
+            report_timeout(p.status, abort_flag, 4);
+        }
+    }
+
+    settle_after_abort(abort_flag);
+    __syncwarp();
+    if (split > 1) {
+        cluster_sync();
+        if (warp >= 2) {
+            const int row = 32 * (warp & 3) + lane;
+            for (int j = rank; j < p.n_few; j += split) {
+                float sum = 0.0f;
+                for (int r = 0; r < split; ++r) sum += ld_cluster_f32(mapa(smem_base + (uint32_t)(j * 128 + row) * 4, (uint32_t)r));
+                few_store(p, row0 + row, j, sum);
+            }
+        }
+        __syncwarp();
+        cluster_sync();   // nobody leaves while another reads its sums
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc<1>(tmem_base, Cfg::kTmem);
     }
 }
 
@@ -422,13 +667,100 @@ static int launch_mx(const MxOperand& a, const MxOperand& b, MxParams p, cudaStr
     return check_cuda(cudaLaunchKernelEx(&lc, mx_matmul_kernel<Cfg>, tm_a, tm_b, tm_sa, tm_sb, p), "mx_matmul launch");
 }
 
+// K split of the kernel for few rows: the fewest passes over the SMs (two CTAs each), counting a fixed cost of about
+// six k-tiles per CTA.
+static int few_split(int tiles, int ktiles)
+{
+    int best = 1;
+    double least = 1e30;
+    for (int s = 1; s <= 8 && s <= ktiles; s *= 2) {
+        const int slots = 2 * sm_count();
+        const double cost = (double)((tiles * s + slots - 1) / slots) * ((double)((ktiles + s - 1) / s) + 6.0);
+        if (cost < least) { least = cost; best = s; }
+    }
+    return best;
+}
+
+template <class Cfg>
+static int launch_few(const MxOperand& a, const MxOperand& b, FewParams p, int64_t K, int split, cudaStream_t stream)
+{
+    CUtensorMap tm_a, tm_b, tm_sa, tm_sb;
+    int rc = make_code_map(&tm_a, a, K, Cfg::kF4, 128, "codes of the long side");
+    if (!rc) rc = make_code_map(&tm_b, b, K, Cfg::kF4, Cfg::kNT, "codes of the few rows");
+    if (!rc) rc = make_scale_map(&tm_sa, a, K, Cfg::kChunks, 1, "scales of the long side");
+    if (!rc) rc = make_scale_map(&tm_sb, b, K, Cfg::kChunks, 1, "scales of the few rows");
+    if (rc) return rc;
+    p.tx_bytes = code_tx(a, Cfg::kF4, 128) + code_tx(b, Cfg::kF4, Cfg::kNT) + 2 * Cfg::kSBytes;
+    p.ktiles = (int)((K + 128 * Cfg::kChunks - 1) / (128 * Cfg::kChunks));
+    {
+        static bool opted_in[64] = {false};
+        int dev = 0;
+        rc = check_cuda(cudaGetDevice(&dev), "cudaGetDevice");
+        if (rc) return rc;
+        if (dev < 0 || dev >= 64 || !opted_in[dev]) {
+            rc = check_cuda(cudaFuncSetAttribute(mx_matmul_few_kernel<Cfg>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes),
+                            "cudaFuncSetAttribute(max dynamic shared memory)");
+            if (rc) return rc;
+            if (dev >= 0 && dev < 64) opted_in[dev] = true;
+        }
+    }
+    const int tiles = (p.n_long + 127) / 128;
+    if (split == 0) split = few_split(tiles, p.ktiles);
+    if (split > p.ktiles) split = 1;
+    cudaLaunchConfig_t lc = {};
+    lc.gridDim = dim3((unsigned)split, (unsigned)tiles);
+    lc.blockDim = dim3(kFewThreads);
+    lc.dynamicSmemBytes = Cfg::kSmemBytes;
+    lc.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)split;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    lc.attrs = attr;
+    lc.numAttrs = 1;
+    return check_cuda(cudaLaunchKernelEx(&lc, mx_matmul_few_kernel<Cfg>, tm_a, tm_b, tm_sa, tm_sb, p), "mx_matmul launch");
+}
+
+template <bool F4>
+static int run_few(const MxOperand& a, const MxOperand& b, const MxParams& p, int split, cudaStream_t stream)
+{
+    const bool swap = p.M <= p.N;   // the few rows are A's
+    const MxOperand& lng = swap ? b : a;
+    const MxOperand& few = swap ? a : b;
+    FewParams f;
+    f.C = p.C;
+    f.stride_long = swap ? 1 : p.ldc;
+    f.stride_few = swap ? p.ldc : 1;
+    f.n_long = (int)lng.rows;
+    f.n_few = (int)few.rows;
+    f.ktiles = 0;
+    f.out = p.out;
+    f.a_format = swap ? p.b_format : p.a_format;
+    f.b_format = swap ? p.a_format : p.b_format;
+    f.tx_bytes = 0;
+    f.status = p.status;
+    f.wait_limit_ns = p.wait_limit_ns;
+    if (f.n_few <= 16) return launch_few<FewCfg<F4, 16, 5>>(lng, few, f, p.K, split, stream);
+    if (f.n_few <= 32) return launch_few<FewCfg<F4, 32, 5>>(lng, few, f, p.K, split, stream);
+    if (f.n_few <= 64) return launch_few<FewCfg<F4, 64, 4>>(lng, few, f, p.K, split, stream);
+    return launch_few<FewCfg<F4, 128, 3>>(lng, few, f, p.K, split, stream);
+}
+
 template <bool F4>
 static int pick_mx(const MxOperand& a, const MxOperand& b, const MxParams& p, const s24_tile_cfg* cfg, cudaStream_t stream)
 {
     int bm = cfg ? cfg->bm : 0, bn = cfg ? cfg->bn : 0;
+    const int few = p.M < p.N ? p.M : p.N, lng = p.M < p.N ? p.N : p.M;
+    // the long side's tiles are the grid's y
+    const bool few_ok = few <= 128 && lng <= 65535 * 128;
+    const int split = cfg ? cfg->split : 0;
+    if (split != 0 && (!few_ok || (split != 1 && split != 2 && split != 4 && split != 8)))
+        return fail(S24_ERR_UNSUPPORTED, "mx_matmul: K can be split 1, 2, 4 or 8 ways, with at most 128 rows on one side (got %d)", split);
+    if (split != 0 || (bm == 0 && bn == 0 && few_ok)) return run_few<F4>(a, b, p, split, stream);
     if (bm == 0) bm = p.M > 128 ? 256 : 128;
     if (bn == 0) bn = bm == 256 && p.N > 128 ? 256 : 128;
-    if (bm == 256 && bn == 256) return launch_mx<MxCfg<2, 256, F4, 6>>(a, b, p, stream);
+    if (bm == 256 && bn == 256) return launch_mx<MxCfg<2, 256, F4, F4 ? 5 : 6>>(a, b, p, stream);
     if (bm == 256 && bn == 128) return launch_mx<MxCfg<2, 128, F4, 8>>(a, b, p, stream);
     if (bm == 128 && bn == 128) return launch_mx<MxCfg<1, 128, F4, 6>>(a, b, p, stream);
     return fail(S24_ERR_UNSUPPORTED, "mx_matmul: no kernel for tile %d x %d (have 256x256, 256x128, 128x128)", bm, bn);

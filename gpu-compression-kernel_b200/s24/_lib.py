@@ -28,7 +28,7 @@ _vp, _i64, _i32, _sz = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_s
 
 
 class TileCfg(ctypes.Structure):
-    _fields_ = [("bm", _i32), ("bn", _i32), ("stages", _i32), ("reserved", _i32)]
+    _fields_ = [("bm", _i32), ("bn", _i32), ("stages", _i32), ("split", _i32)]
 
 
 SIGNATURES = {

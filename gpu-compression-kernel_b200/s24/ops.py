@@ -227,7 +227,7 @@ def _tile_cfg(manual_config: Optional[dict]):
     if not manual_config:
         return None
     # the ring depth ("buffers" in the reference's configs) is fixed per tile shape here
-    cfg = L.TileCfg(int(manual_config.get("BM", 0)), int(manual_config.get("BN", 0)), 0, 0)
+    cfg = L.TileCfg(int(manual_config.get("BM", 0)), int(manual_config.get("BN", 0)), 0, int(manual_config.get("SPLIT", 0)))
     return ctypes.byref(cfg)
 
 

@@ -192,6 +192,7 @@ def _operand(s24, r, k, fmt, seed, exact):
 
 
 PAIRS = [("mxfp4", "mxfp4"), ("mxfp8", "mxfp8"), ("mxfp8", "mxfp4"), ("mxfp4", "mxfp8")]
+SPLITS = [{"SPLIT": 1}, {"SPLIT": 2}, {"SPLIT": 4}, {"SPLIT": 8}]    # the kernel for few rows, K split over that many CTAs
 TILES = [None, {"BM": 128, "BN": 128}, {"BM": 256, "BN": 128}, {"BM": 256, "BN": 256}]
 
 
@@ -205,7 +206,7 @@ def test_product_is_exact_where_sums_are(s24, m, n, k, fa, fb):
     a, sa, va = _operand(s24, m, k, fa, 1000 * m + k, True)
     b, sb, vb = _operand(s24, n, k, fb, 1000 * n + k + 1, True)
     want = torch.from_numpy(va) @ torch.from_numpy(vb).t()      # below 2^6 * 2048 * ..., whole multiples of 2^-6: exact in fp32
-    for tile in TILES:
+    for tile in TILES + (SPLITS if min(m, n) <= 128 else []):
         got = s24.mx_matmul(a, sa, b, sb, out_dtype=torch.float32, manual_config=tile)
         assert torch.equal(got.cpu().double(), want), f"tile {tile}: {(got.cpu().double() != want).sum()} of {want.numel()} differ"
     for out in (torch.bfloat16, torch.float16):
