@@ -98,12 +98,12 @@ struct MxParams {
     int out;                 // S24_FP16 / S24_BF16 / S24_FP32
     uint32_t a_format, b_format;
     uint32_t tx_bytes;       // bytes a CTA's copies of one k-tile deliver
-    int wide;                // rows of C allow 16-byte stores
+    int wide;                // rows of C allow 32-byte stores
     int* status;
     unsigned long long wait_limit_ns;
 };
 
-constexpr int kStorePitch = 17;                              // words: 16 of a row and one against bank conflicts
+constexpr int kStorePitch = 9;                               // words: 8 of a row and one against bank conflicts
 constexpr int kStoreWarpBytes = 32 * kStorePitch * 4;
 
 template <int G, int BN, bool F4, int ST>
@@ -131,9 +131,16 @@ struct MxCfg {
     static_assert(8 * (2 * ST + 2) + 16 <= 256, "barrier block");
 };
 
-// 32 rows (one per lane) x 32 accumulator columns to C.  Rows that allow 16-byte stores take them straight from
-// the registers (64 or 128 bytes per lane); others go through 2 KB of shared memory, so that 16 lanes write one
-// row's 64 bytes instead of every lane its own row in elements.
+__device__ __forceinline__ void store_sector(void* p, const uint32_t* q)
+{
+    asm volatile("st.global.L1::no_allocate.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(q[0]), "r"(q[1]), "r"(q[2]), "r"(q[3]),
+                 "r"(q[4]), "r"(q[5]), "r"(q[6]), "r"(q[7])
+                 : "memory");
+}
+
+// 32 rows (one per lane) x 32 accumulator columns to C.  Rows that allow 32-byte stores take them straight from
+// the registers, a whole sector each (8192^3: 199 us against 203 with 16-byte stores); others go through 1 KB of shared memory, so that 8 lanes write 32 bytes
+// of one row instead of every lane its own row in elements.
 __device__ __forceinline__ void mx_store32(const MxParams& p, int row0, int col, const uint32_t (&r)[32], uint32_t staging, int lane)
 {
     if (row0 >= p.M || col >= p.N) return;   // the same for the whole warp
@@ -149,35 +156,35 @@ __device__ __forceinline__ void mx_store32(const MxParams& p, int row0, int col,
     if (p.wide && col + 32 <= p.N) {
         const int64_t at = (int64_t)(row0 + lane) * p.ldc + col;
         if (row0 + lane < p.M) {
-            uint4* c = reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.C) + at * (f32 ? 4 : 2));
+            uint8_t* c = static_cast<uint8_t*>(p.C) + at * (f32 ? 4 : 2);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) c[i] = make_uint4(q[4 * i], q[4 * i + 1], q[4 * i + 2], q[4 * i + 3]);
+            for (int i = 0; i < 2; ++i) store_sector(c + 32 * i, &q[8 * i]);
             if (f32) {
 #pragma unroll
-                for (int i = 4; i < 8; ++i) c[i] = make_uint4(q[4 * i], q[4 * i + 1], q[4 * i + 2], q[4 * i + 3]);
+                for (int i = 2; i < 4; ++i) store_sector(c + 32 * i, &q[8 * i]);
             }
         }
         return;
     }
-    const int word = lane & 15;
+    const int word = lane & 7;
 #pragma unroll
-    for (int part = 0; part < 2; ++part) {
-        if (part == 1 && !f32) break;
+    for (int part = 0; part < 4; ++part) {
+        if (part >= 2 && !f32) break;
         __syncwarp();
 #pragma unroll
-        for (int i = 0; i < 16; ++i) st_shared_u32(staging + (uint32_t)(lane * kStorePitch + i) * 4, q[16 * part + i]);
+        for (int i = 0; i < 8; ++i) st_shared_u32(staging + (uint32_t)(lane * kStorePitch + i) * 4, q[8 * part + i]);
         __syncwarp();
 #pragma unroll 4
-        for (int i = 0; i < 16; ++i) {
-            const int rr = 2 * i + (lane >> 4), row = row0 + rr;
+        for (int i = 0; i < 8; ++i) {
+            const int rr = 4 * i + (lane >> 3), row = row0 + rr;
             uint32_t v;
             asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(staging + (uint32_t)(rr * kStorePitch + word) * 4) : "memory");
             if (row >= p.M) continue;
             if (f32) {
-                const int c = col + 16 * part + word;
+                const int c = col + 8 * part + word;
                 if (c < p.N) static_cast<float*>(p.C)[(int64_t)row * p.ldc + c] = __uint_as_float(v);
             } else {
-                const int c = col + 2 * word;
+                const int c = col + 2 * (8 * part + word);
                 uint16_t* dst = static_cast<uint16_t*>(p.C) + (int64_t)row * p.ldc + c;
                 if (c + 1 < p.N && (reinterpret_cast<uintptr_t>(dst) & 3u) == 0) {
                     *reinterpret_cast<uint32_t*>(dst) = v;
@@ -429,10 +436,10 @@ struct FewCfg {
     static_assert(2 * (kSmemBytes + 1024) <= 233472, "two CTAs per SM");
 };
 
-__device__ __forceinline__ float ld_cluster_f32(uint32_t cluster_addr)
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t cluster_addr)
 {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr) : "memory");
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(cluster_addr));
     return v;
 }
 
@@ -443,6 +450,30 @@ __device__ __forceinline__ void few_store(const FewParams& p, int i, int j, floa
     if (p.out == S24_FP32) static_cast<float*>(p.C)[at] = v;
     else if (p.out == S24_BF16) static_cast<__nv_bfloat16*>(p.C)[at] = __float2bfloat16_rn(v);
     else static_cast<__half*>(p.C)[at] = __float2half_rn(v);
+}
+
+// This CTA's share of the columns (every S-th), four rows per thread and step: sums of the S partial sums.  The S loads
+// of a step do not wait for one another (one at a time cost 35 us of 75 with 128 rows and S = 2).
+template <int S>
+__device__ __forceinline__ void few_reduce(const FewParams& p, uint32_t sums, int rank, int row0, int thread)
+{
+    for (int it = thread; it < 32 * ((p.n_few - rank + S - 1) / S); it += 128) {
+        const int j = rank + S * (it >> 5), row = (it & 31) * 4;
+        float4 v[S];
+#pragma unroll
+        for (int r = 0; r < S; ++r) v[r] = ld_cluster_f32x4(mapa(sums + (uint32_t)(j * 128 + row) * 4, (uint32_t)r));
+#pragma unroll
+        for (int r = 1; r < S; ++r) {
+            v[0].x += v[r].x;
+            v[0].y += v[r].y;
+            v[0].z += v[r].z;
+            v[0].w += v[r].w;
+        }
+        few_store(p, row0 + row, j, v[0].x);
+        few_store(p, row0 + row + 1, j, v[0].y);
+        few_store(p, row0 + row + 2, j, v[0].z);
+        few_store(p, row0 + row + 3, j, v[0].w);
+    }
 }
 
 template <class Cfg>
@@ -576,12 +607,10 @@ mx_matmul_few_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
     if (split > 1) {
         cluster_sync();
         if (warp >= 2) {
-            const int row = 32 * (warp & 3) + lane;
-            for (int j = rank; j < p.n_few; j += split) {
-                float sum = 0.0f;
-                for (int r = 0; r < split; ++r) sum += ld_cluster_f32(mapa(smem_base + (uint32_t)(j * 128 + row) * 4, (uint32_t)r));
-                few_store(p, row0 + row, j, sum);
-            }
+            const int thread = (int)threadIdx.x - 64;
+            if (split == 2) few_reduce<2>(p, smem_base, rank, row0, thread);
+            else if (split == 4) few_reduce<4>(p, smem_base, rank, row0, thread);
+            else few_reduce<8>(p, smem_base, rank, row0, thread);
         }
         __syncwarp();
         cluster_sync();   // nobody leaves while another reads its sums
@@ -667,17 +696,15 @@ static int launch_mx(const MxOperand& a, const MxOperand& b, MxParams p, cudaStr
     return check_cuda(cudaLaunchKernelEx(&lc, mx_matmul_kernel<Cfg>, tm_a, tm_b, tm_sa, tm_sb, p), "mx_matmul launch");
 }
 
-// K split of the kernel for few rows: the fewest passes over the SMs (two CTAs each), counting a fixed cost of about
-// six k-tiles per CTA.
+// K split of the kernel for few rows: as many CTAs as find room at once (two per SM), but a second CTA on an SM only
+// where each still has 8 k-tiles.  Measured, 4-bit weight and 8-bit rows: 32 x 8192 x 8192 18.5 / 13.7 / 12.1 / 17.3 us
+// with 1 / 2 / 4 / 8 CTAs sharing K (64 tiles: 4 fill the SMs), 1 x 4096 x 4096 8.5 / 6.6 / 5.4 / 6.6 (32 tiles: 8 would
+// be a second CTA with 4 k-tiles), 4 x 28672 x 8192 24.3 / 28.8 / 34.7 / 46.8 (224 tiles: 1).
 static int few_split(int tiles, int ktiles)
 {
     int best = 1;
-    double least = 1e30;
-    for (int s = 1; s <= 8 && s <= ktiles; s *= 2) {
-        const int slots = 2 * sm_count();
-        const double cost = (double)((tiles * s + slots - 1) / slots) * ((double)((ktiles + s - 1) / s) + 6.0);
-        if (cost < least) { least = cost; best = s; }
-    }
+    for (int s = 2; s <= 8 && s <= ktiles; s *= 2)
+        if (tiles * s <= sm_count() || (tiles * s <= 2 * sm_count() && ktiles / s >= 8)) best = s;
     return best;
 }
 
@@ -747,20 +774,42 @@ static int run_few(const MxOperand& a, const MxOperand& b, const MxParams& p, in
     return launch_few<FewCfg<F4, 128, 3>>(lng, few, f, p.K, split, stream);
 }
 
+// Which kernel and tile: the least of a time that is a fixed part (launch, first copies, last epilogue) and one per k-tile
+// and pass over the SMs, in microseconds as measured with the operands in L2 at 256 rows and K of 512 to 16384.  What the
+// memory bounds, it bounds for all of them alike.  Measured against it (tiles 256 x 256, 256 x 128, 128 x 128):
+// 256 x 8192 x 8192 4-bit 17.4 / 13.6 / 14.7 us, 512 x 8192 x 8192 8-by-4-bit 28.0 / 30.5 / 34.6, 160 x 1000 x 1024 8-bit
+// 20.5 / 13.7 / 13.1; few rows, against the best tile: 64 x 28672 x 8192 30.7 / 35.7, 128 x 28672 x 8192 39.1 / 36.7,
+// 128 x 4096 x 16384 18.4 / 26.6.
 template <bool F4>
 static int pick_mx(const MxOperand& a, const MxOperand& b, const MxParams& p, const s24_tile_cfg* cfg, cudaStream_t stream)
 {
     int bm = cfg ? cfg->bm : 0, bn = cfg ? cfg->bn : 0;
     const int few = p.M < p.N ? p.M : p.N, lng = p.M < p.N ? p.N : p.M;
-    // the long side's tiles are the grid's y
-    const bool few_ok = few <= 128 && lng <= 65535 * 128;
+    const bool few_ok = few <= 128 && lng <= 65535 * 128;   // the long side's tiles are the grid's y
     const int split = cfg ? cfg->split : 0;
     if (split != 0 && (!few_ok || (split != 1 && split != 2 && split != 4 && split != 8)))
         return fail(S24_ERR_UNSUPPORTED, "mx_matmul: K can be split 1, 2, 4 or 8 ways, with at most 128 rows on one side (got %d)", split);
-    if (split != 0 || (bm == 0 && bn == 0 && few_ok)) return run_few<F4>(a, b, p, split, stream);
-    if (bm == 0) bm = p.M > 128 ? 256 : 128;
-    if (bn == 0) bn = bm == 256 && p.N > 128 ? 256 : 128;
-    if (bm == 256 && bn == 256) return launch_mx<MxCfg<2, 256, F4, F4 ? 5 : 6>>(a, b, p, stream);
+    if (split != 0) return run_few<F4>(a, b, p, split, stream);
+    if (bm == 0 && bn == 0) {
+        if (few_ok && few <= 64) return run_few<F4>(a, b, p, 0, stream);
+        struct Tile { int bm, bn, units; double fixed, per_ktile, per_pass; };
+        const Tile tiles[3] = {{256, 256, sm_count() / 2, 5.7, 0.29, 0.0}, {256, 128, sm_count() / 2, 4.7, 0.185, 0.6}, {128, 128, sm_count(), 4.3, 0.21, 0.6}};
+        const double ktiles = (double)((p.K + (F4 ? 255 : 127)) / (F4 ? 256 : 128));
+        double least = 1e30;
+        for (const Tile& t : tiles) {
+            const int64_t n = (((int64_t)p.M + t.bm - 1) / t.bm) * (((int64_t)p.N + t.bn - 1) / t.bn);
+            const double passes = (double)((n + t.units - 1) / t.units);
+            const double time = t.fixed + passes * ktiles * t.per_ktile + (passes - 1) * t.per_pass;
+            if (time < least) { least = time; bm = t.bm; bn = t.bn; }
+        }
+        if (few_ok) {
+            const int n = (lng + 127) / 128, s = few_split(n, (int)ktiles);
+            if (n * s <= 2 * sm_count() && 6.5 + ktiles / s * (n * s > sm_count() ? 0.72 : 0.36) < least) return run_few<F4>(a, b, p, s, stream);
+        }
+    }
+    if (bm == 0) bm = bn == 256 || p.M > 128 ? 256 : 128;
+    if (bn == 0) bn = 128;
+    if (bm == 256 && bn == 256) return launch_mx<MxCfg<2, 256, F4, 6>>(a, b, p, stream);
     if (bm == 256 && bn == 128) return launch_mx<MxCfg<2, 128, F4, 8>>(a, b, p, stream);
     if (bm == 128 && bn == 128) return launch_mx<MxCfg<1, 128, F4, 6>>(a, b, p, stream);
     return fail(S24_ERR_UNSUPPORTED, "mx_matmul: no kernel for tile %d x %d (have 256x256, 256x128, 128x128)", bm, bn);
@@ -808,7 +857,7 @@ extern "C" int s24_mx_matmul(const void* a, const void* a_scales, const void* b,
     p.a_format = both4 ? 1u : fmt_a == S24_MXFP4 ? 5u : 0u;
     p.b_format = both4 ? 1u : fmt_b == S24_MXFP4 ? 5u : 0u;
     p.tx_bytes = 0;
-    p.wide = aligned(C, 16) && (ldc * esz) % 16 == 0;
+    p.wide = aligned(C, 32) && (ldc * esz) % 32 == 0;
     p.status = status;
     p.wait_limit_ns = kWaitTimeoutNs;
     const MxOperand oa = {a, a_scales, M, lda, fmt_a}, ob = {b, b_scales, N, ldb, fmt_b};

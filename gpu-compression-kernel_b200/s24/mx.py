@@ -14,7 +14,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib as L
-from .ops import _after_gemm, _on_device, _p, _require_cuda, _stream, _tile_cfg
+from .ops import _NVTX, _after_gemm, _on_device, _require_cuda, _tile_cfg
 
 _DT = {torch.float16: L.FP16, torch.bfloat16: L.BF16, torch.float32: L.FP32}
 _FMT = {"mxfp4": L.MXFP4, "mxfp8": L.MXFP8}
@@ -22,19 +22,44 @@ _SCALES = {"rows": L.SCALES_ROWS, "tc": L.SCALES_TC}
 _SCALE_TYPES = (torch.uint8, torch.float8_e8m0fnu)
 
 
+# A decoding step's calls are a few microseconds long on the GPU, so the way to the launch is kept short here:
+# device checks on indexes, the stream's handle without a Stream object, plain integers for the pointers.
+
+def _device_of(*ts: Optional[torch.Tensor]) -> int:
+    d = ts[0].get_device()
+    for t in ts:
+        if t is not None and t.get_device() != d or d < 0:
+            _require_cuda(*ts)   # says which and why
+    return d
+
+
+def _call(name: str, t: torch.Tensor, device: int, *args) -> None:
+    """library call `name` on t's device and its current stream"""
+    fn = getattr(L.lib(), name)
+    if torch._C._cuda_getDevice() == device and not _NVTX:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(device))
+    else:
+        with _on_device(t, name[4:]):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(device))
+    if rc != L.OK:
+        L.check(rc)
+
+
 def mx_scales_numel(R: int, K: int) -> int:
     """bytes of a tensor-core-order scale buffer for an (R, K) matrix"""
-    return int(L.lib().s24_mx_scales_tc_bytes(R, K))
+    return -(-R // 128) * -(-K // 128) * 512 if R > 0 and K > 0 else 0
 
 
 def _rows_of(t: torch.Tensor) -> Tuple[int, int]:
-    if t.dim() < 1:
+    shape = t.shape
+    if len(shape) == 2:
+        return shape
+    if not shape:
         raise RuntimeError("expected a tensor of at least one dimension")
-    k = t.shape[-1]
     r = 1
-    for n in t.shape[:-1]:
+    for n in shape[:-1]:
         r *= n
-    return r, k
+    return r, shape[-1]
 
 
 def _matrix(t: torch.Tensor, R: int, step: int) -> Tuple[torch.Tensor, int]:
@@ -43,11 +68,16 @@ def _matrix(t: torch.Tensor, R: int, step: int) -> Tuple[torch.Tensor, int]:
     width = t.shape[-1]
     if t.dim() != 2:
         t = t.reshape(R, width)
-    size = t.element_size()
-    stride = t.stride(0) if R > 1 else width
-    if t.stride(1) != 1 and width > 1 or stride < width or stride * size % step or t.data_ptr() % step:
+    stride, inner = t.stride()
+    if R == 1:
+        stride = width
+    if inner != 1 and width > 1 or stride < width or stride * t.element_size() % step or t.data_ptr() % step:
         t, stride = t.clone(memory_format=torch.contiguous_format), width
     return t, stride
+
+
+def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
 
 
 def _check_fmt(fmt: str) -> int:
@@ -104,12 +134,11 @@ def mx_quantize(x: torch.Tensor, fmt: str = "mxfp4", want_rows: bool = True, wan
     if x.dtype not in _DT:
         raise RuntimeError(f"Invalid datatype {x.dtype} of dense matrix")
     _check_k(K)
-    _require_cuda(x)
+    d = _device_of(x)
     codes, scales, tc = _new_quantized(x.shape[:-1], R, K, f, want_rows, want_tc, x.device)
     if R * K:
         m, ld = _matrix(x, R, 16)
-        with _on_device(x):
-            L.check(L.lib().s24_mx_quantize(_p(m), R, K, ld, _DT[x.dtype], f, _p(codes), _p(scales), _p(tc), _stream(x)))
+        _call("s24_mx_quantize", x, d, m.data_ptr(), R, K, ld, _DT[x.dtype], f, codes.data_ptr(), _ptr(scales), _ptr(tc))
     return codes, scales, tc
 
 
@@ -119,12 +148,11 @@ def mx_dequantize(codes: torch.Tensor, scales: torch.Tensor, layout: str = "rows
     if dtype not in _DT:
         raise RuntimeError(f"Invalid datatype {dtype} of dense matrix")
     _check_scales(scales, layout, R, K)
-    _require_cuda(codes, scales)
+    d = _device_of(codes, scales)
     out = torch.empty((*codes.shape[:-1], K), dtype=dtype, device=codes.device)
     if R * K:
         c = codes if codes.is_contiguous() and codes.data_ptr() % 16 == 0 else codes.clone(memory_format=torch.contiguous_format)
-        with _on_device(codes):
-            L.check(L.lib().s24_mx_dequantize(_p(c), _p(scales), _SCALES[layout], _p(out), R, K, f, _DT[dtype], _stream(codes)))
+        _call("s24_mx_dequantize", codes, d, c.data_ptr(), scales.data_ptr(), _SCALES[layout], out.data_ptr(), R, K, f, _DT[dtype])
     return out
 
 
@@ -134,12 +162,11 @@ def mx_scales_convert(scales: torch.Tensor, from_layout: str, to_layout: str, R:
     _check_scales(scales, from_layout, R, K)
     if to_layout not in _SCALES or to_layout == from_layout:
         raise ValueError(f"cannot convert scales from {from_layout!r} to {to_layout!r}")
-    _require_cuda(scales)
+    d = _device_of(scales)
     shape = (R, K // 32) if to_layout == "rows" else (mx_scales_numel(R, K),)
     out = torch.empty(shape, dtype=torch.uint8, device=scales.device)
     if R * K:
-        with _on_device(scales):
-            L.check(L.lib().s24_mx_scales_convert(_p(scales), _SCALES[from_layout], _p(out), _SCALES[to_layout], R, K, _stream(scales)))
+        _call("s24_mx_scales_convert", scales, d, scales.data_ptr(), _SCALES[from_layout], out.data_ptr(), _SCALES[to_layout], R, K)
     return out
 
 
@@ -162,16 +189,15 @@ def mx_rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residu
         raise RuntimeError(f"`residual` must be a {tuple(x.shape)} {x.dtype} tensor, got {tuple(residual.shape)} {residual.dtype}")
     if K > L.MX_NORM_MAX_K:
         raise RuntimeError(f"rows of at most {L.MX_NORM_MAX_K} elements (got {K})")
-    _require_cuda(x, weight, residual)
+    d = _device_of(x, weight, residual)
     codes, scales, tc = _new_quantized(x.shape[:-1], R, K, f, want_rows, want_tc, x.device)
     h = x if residual is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
     if R * K:
         m, ldx = _matrix(x, R, 16)
         r, ldr = (None, 0) if residual is None else _matrix(residual, R, 16)
         w, _ = _matrix(weight, 1, 16)
-        with _on_device(x):
-            L.check(L.lib().s24_mx_rms_norm(_p(m), _p(r), _p(w), _p(None if residual is None else h), R, K, ldx, ldr, float(eps),
-                                            _DT[x.dtype], f, _p(codes), _p(scales), _p(tc), _stream(x)))
+        _call("s24_mx_rms_norm", x, d, m.data_ptr(), _ptr(r), w.data_ptr(), None if residual is None else h.data_ptr(), R, K, ldx, ldr, eps,
+              _DT[x.dtype], f, codes.data_ptr(), _ptr(scales), _ptr(tc))
     return codes, scales, tc, h
 
 
@@ -195,7 +221,7 @@ def mx_matmul(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_scales
         raise RuntimeError(f"Invalid datatype {out_dtype} of the product")
     _check_scales(a_scales, "tc", M, K)
     _check_scales(b_scales, "tc", N, K)
-    _require_cuda(a, a_scales, b, b_scales, out)
+    d = _device_of(a, a_scales, b, b_scales, out)
     if out is None:
         c = torch.empty((*a.shape[:-1], N), dtype=out_dtype, device=a.device)
         ldc = N
@@ -207,8 +233,7 @@ def mx_matmul(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_scales
     if M * N:
         ma, lda = _matrix(a, M, 32 if fa == L.MXFP4 != fb else 16)
         mb, ldb = _matrix(b, N, 32 if fb == L.MXFP4 != fa else 16)
-        with _on_device(a):
-            L.check(L.lib().s24_mx_matmul(_p(ma), _p(a_scales), _p(mb), _p(b_scales), _p(c), M, N, K, lda, ldb, ldc, fa, fb, _DT[out_dtype],
-                                          _tile_cfg(manual_config), _stream(a)))
-            _after_gemm(a)
+        _call("s24_mx_matmul", a, d, ma.data_ptr(), a_scales.data_ptr(), mb.data_ptr(), b_scales.data_ptr(), c.data_ptr(), M, N, K, lda, ldb,
+              ldc, fa, fb, _DT[out_dtype], _tile_cfg(manual_config))
+        _after_gemm(a)
     return c

@@ -34,10 +34,11 @@ _NVTX = os.environ.get("S24_NVTX", "0") not in ("", "0")
 class _on_device:
     """`with _on_device(t):` makes t's device current for the library call; a no-op (and much
     cheaper than torch.cuda.device) when it already is, which is the common case"""
-    __slots__ = ("idx", "prev", "ranged")
+    __slots__ = ("idx", "prev", "ranged", "name")
 
-    def __init__(self, t: torch.Tensor):
+    def __init__(self, t: torch.Tensor, name: Optional[str] = None):
         self.idx = t.device.index
+        self.name = name
         self.prev = None
         self.ranged = False
 
@@ -47,7 +48,7 @@ class _on_device:
             self.prev = cur
             torch.cuda.set_device(self.idx)
         if _NVTX:
-            torch.cuda.nvtx.range_push("s24." + sys._getframe(1).f_code.co_name)
+            torch.cuda.nvtx.range_push("s24." + (self.name or sys._getframe(1).f_code.co_name))
             self.ranged = True
 
     def __exit__(self, *exc):
