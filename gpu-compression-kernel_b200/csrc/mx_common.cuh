@@ -141,6 +141,43 @@ __device__ __forceinline__ uint32_t pack2(float a, float b)
     }
 }
 
+// two fp32 numbers in one 64-bit register pair, and operations on both at once
+struct Pair {
+    uint64_t v;
+};
+__device__ __forceinline__ Pair make_pair(float a, float b)
+{
+    Pair p;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(p.v) : "f"(a), "f"(b));
+    return p;
+}
+__device__ __forceinline__ float2 split(Pair p)
+{
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p.v));
+    return f;
+}
+__device__ __forceinline__ Pair operator*(Pair a, Pair b)
+{
+    Pair r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ Pair operator+(Pair a, Pair b)
+{
+    Pair r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+
+// largest magnitude of three, NaN if one is
+__device__ __forceinline__ float max_magnitude(float a, float b, float c)
+{
+    float r;
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
 __device__ __forceinline__ uint32_t magnitude_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
 
 }  // namespace mx
