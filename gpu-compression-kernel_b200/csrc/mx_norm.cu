@@ -55,203 +55,197 @@ struct NormParams {
     double eps, inv_k;
 };
 
-// eight values of y, rounded to odd
+
+// The exact form of one value of y = h * rinv * w with rinv = rhi + rlo, rounded to odd.  h and w are read again: this runs
+// for one element in 10^5, and registers that it kept would be the common path's.
 template <int DT>
-__device__ __forceinline__ void norm_exact(const uint32_t (&h)[4], const uint32_t (&w)[4], float rhi, float rlo, Pair (&y)[4])
+__device__ __forceinline__ float norm_exact(const uint8_t* h, const uint8_t* w, float rhi, float rlo)
 {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 a = unpack2<DT>(h[i]), c = unpack2<DT>(w[i]);
-        float o[2];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const float hv = j ? a.y : a.x, wv = j ? c.y : c.x;
-            const float t = hv * rhi;
-            const float t_err = fmaf(hv, rlo, fmaf(hv, rhi, -t));
-            const float v = t * wv;
-            o[j] = round_to_odd(v, fmaf(t_err, wv, fmaf(t, wv, -v)));
-        }
-        y[i] = make_pair(o[0], o[1]);
-    }
+    const float hv = unpack2<DT>(*reinterpret_cast<const uint16_t*>(h)).x, wv = unpack2<DT>(*reinterpret_cast<const uint16_t*>(w)).x;
+    const float t = hv * rhi;
+    const float t_err = fmaf(hv, rlo, fmaf(hv, rhi, -t));
+    const float v = t * wv;
+    return round_to_odd(v, fmaf(t_err, wv, fmaf(t, wv, -v)));
 }
 
-// codes of eight values (four pairs) times up
+// codes of a piece times up
 template <int FMT>
-__device__ __forceinline__ void encode8(const Pair (&y)[4], float up, uint32_t (&c)[FMT == S24_MXFP4 ? 1 : 2])
+__device__ __forceinline__ void encode_piece(const Pair (&y)[8], float up, uint32_t (&c)[FMT == S24_MXFP4 ? 2 : 4])
 {
-    float u[8];
+    float u[16];
     const Pair up2 = make_pair(up, up);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 8; ++i) {
         const float2 f = split(y[i] * up2);
         u[2 * i] = f.x;
         u[2 * i + 1] = f.y;
     }
-    if constexpr (FMT == S24_MXFP4) {
-        c[0] = to_e2m1x8(u);
-    } else {
-        c[0] = to_e4m3x4(u);
-        c[1] = to_e4m3x4(u + 4);
-    }
+#pragma unroll
+    for (int i = 0; i < (FMT == S24_MXFP4 ? 2 : 4); ++i) c[i] = FMT == S24_MXFP4 ? to_e2m1x8(u + 8 * i) : to_e4m3x4(u + 4 * i);
 }
 
-// bits of the largest magnitude of eight values; a NaN among them gives the bits of a NaN
-__device__ __forceinline__ uint32_t max8(const Pair (&y)[4])
-{
-    const float2 a = split(y[0]), b = split(y[1]), c = split(y[2]), d = split(y[3]);
-    return __float_as_uint(max_magnitude(max_magnitude(a.x, a.y, b.x), max_magnitude(b.y, c.x, c.y), max_magnitude(d.x, d.y, 0.0f)));
-}
-
-// over the four threads that hold a block
-__device__ __forceinline__ uint32_t max_of_block(uint32_t m)
-{
-    const uint32_t mask = 0xFu << (threadIdx.x & 28);
-    m = max(m, __shfl_xor_sync(mask, m, 1));
-    return max(m, __shfl_xor_sync(mask, m, 2));
-}
-
-// TPR threads per row, four to a block of 32 elements: thread t takes elements 8 t .. 8 t + 7 and every 8 TPR further, NC
-// pieces in all, so that a warp's loads and stores are whole lines (with a block per thread the same kernel took 117 us
-// instead of 78 at 8192 x 8192 with a residual: 18 accesses of 16 lines each per warp).  A row stays in registers between
-// the sum and the quantisation: x and the residual are read once.
+// A row belongs to TPR threads (4 to 32) of a CTA of 128, or, with TPR = 0, to a whole CTA of as many warps as it takes.
+// Two threads hold a block of 32 elements: thread t takes elements 16 t .. 16 t + 15 and every 16 TPR further, NC pieces in
+// all, 32 bytes each, so that a warp's accesses are whole lines.  The row stays in registers between the sum and the
+// quantisation: x and the residual are read once.
+//
+// What bounds it: with a residual the 7.03 bytes an element (8 bits out), without one the instructions, about 14 an
+// element.  Measured, 8192 x 8192 bf16 with a residual: a block per thread 117 us, an eighth of a block (8 elements) per
+// thread 74 to 80 us with 22 to 28 instructions an element; 4099 x 6144 fp16 to 4 bits 34, 25 to 27 us.
 template <int DT, int FMT, int TPR, int NC>
-__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR)
+__global__ void __launch_bounds__(TPR == 0 ? 1024 : 128, TPR == 0 ? 1 : 8)
 mx_rms_norm_kernel(const NormParams p)
 {
-    constexpr int kThreads = TPR < 128 ? 128 : TPR;
-    constexpr int kRows = kThreads / TPR;
-    constexpr int kWarps = TPR / 32;
-    const uint32_t sub = threadIdx.x % TPR;
-    const uint32_t r = blockIdx.x * kRows + threadIdx.x / TPR;
-    const uint32_t pieces = r < p.R ? p.KB * 4 : 0;   // of eight elements
+    const uint32_t tpr = TPR == 0 ? blockDim.x : TPR;
+    const uint32_t sub = TPR == 0 ? threadIdx.x : threadIdx.x % (TPR == 0 ? 1 : TPR);
+    const uint32_t r = TPR == 0 ? blockIdx.x : blockIdx.x * (128 / (TPR == 0 ? 1 : TPR)) + threadIdx.x / (TPR == 0 ? 1 : TPR);
+    const uint32_t pieces = r < p.R ? p.KB * 2 : 0;
 
-    uint32_t h[NC][4];
+    uint32_t h[NC][8];
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-        const uint32_t at = sub + c * TPR;
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (at < pieces) v = reinterpret_cast<const uint4*>(p.x + (int64_t)r * p.x_row_bytes)[at];
-        h[c][0] = v.x; h[c][1] = v.y; h[c][2] = v.z; h[c][3] = v.w;
+        const uint32_t at = sub + c * tpr;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) h[c][i] = 0u;
+        if (at < pieces) load32(p.x + (int64_t)r * p.x_row_bytes + at * 32, h[c]);
     }
     if (p.residual != nullptr) {
-        uint4 v[NC];
+        uint32_t v[NC][8];
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            const uint32_t at = sub + c * TPR;
-            v[c] = make_uint4(0u, 0u, 0u, 0u);
-            if (at < pieces) v[c] = reinterpret_cast<const uint4*>(p.residual + (int64_t)r * p.r_row_bytes)[at];
+            const uint32_t at = sub + c * tpr;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[c][i] = 0u;
+            if (at < pieces) load32(p.residual + (int64_t)r * p.r_row_bytes + at * 32, v[c]);
         }
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            const uint32_t at = sub + c * TPR;
-            const uint32_t u[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
+            const uint32_t at = sub + c * tpr;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < 8; ++i) {
                 // the fp32 sum of two 16-bit values rounds to 16 bits as the exact sum does
                 // (24 bits are at least twice the type's plus two)
-                const float2 a = unpack2<DT>(h[c][i]), b = unpack2<DT>(u[i]);
+                const float2 a = unpack2<DT>(h[c][i]), b = unpack2<DT>(v[c][i]);
                 const float2 f = split(make_pair(a.x, a.y) + make_pair(b.x, b.y));
                 h[c][i] = mx::pack2<DT>(f.x, f.y);
             }
-            if (at < pieces) reinterpret_cast<uint4*>(p.h + (int64_t)r * p.KB * 64)[at] = make_uint4(h[c][0], h[c][1], h[c][2], h[c][3]);
+            if (at < pieces) store32(p.h + (int64_t)r * (p.KB * 64) + at * 32, h[c]);
         }
     }
-    double sum = 0.0;
+    double s0 = 0.0, s1 = 0.0;   // two chains: one alone waits for itself
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 8; ++i) {
             const float2 a = unpack2<DT>(h[c][i]);
-            sum = fma((double)a.x, (double)a.x, sum);
-            sum = fma((double)a.y, (double)a.y, sum);
+            s0 = fma((double)a.x, (double)a.x, s0);
+            s1 = fma((double)a.y, (double)a.y, s1);
         }
     }
+    double sum = s0 + s1;
 #pragma unroll
-    for (int o = (TPR < 32 ? TPR : 32) / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-    if constexpr (kWarps > 1) {
-        __shared__ double part[kRows][kWarps];
-        const uint32_t own = threadIdx.x / TPR;
-        if ((threadIdx.x & 31) == 0) part[own][sub >> 5] = sum;
+    for (int o = (TPR == 0 ? 32 : TPR) / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+    if constexpr (TPR == 0) {
+        __shared__ double part[32];
+        if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = sum;
         __syncthreads();
-        sum = 0.0;
-#pragma unroll
-        for (int i = 0; i < kWarps; ++i) sum += part[own][i];
+        sum = part[0];
+        for (uint32_t i = 1; i < blockDim.x >> 5; ++i) sum += part[i];
     }
     const double rinv = inverse_sqrt(sum * p.inv_k + p.eps);
     const float rhi = (float)rinv;
     const float rlo = (float)(rinv - (double)rhi);
 
+    uint8_t* codes = p.codes + (int64_t)r * (p.KB * Format<FMT>::kBytes);
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-        const uint32_t at = sub + c * TPR, kb = at >> 2;
-        uint32_t s = 0;
-        if (at < pieces) {   // the same for the four threads of a block
-            const uint4 q = reinterpret_cast<const uint4*>(p.weight)[at];
-            const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-            Pair y[4];
+        const uint32_t at = sub + c * tpr, kb = at >> 1;
+        const bool ok = at < pieces;   // the same for the two threads of a block
+        uint32_t w[8];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float2 a = unpack2<DT>(h[c][i]), b = unpack2<DT>(w[i]);
-                y[i] = make_pair(a.x, a.y) * make_pair(rhi, rhi) * make_pair(b.x, b.y);
-            }
-            uint32_t amax = max_of_block(max8(y));
-            // a power of two too near to tell the scale, or numbers too small for fp32's own rounding
-            bool exact = ((amax + 8u) & 0x7FFFFFu) < 16u || amax - 1u < 0x0E800000u;
-            if (exact) {
-                norm_exact<DT>(h[c], w, rhi, rlo, y);
-                amax = max_of_block(max8(y));
-            }
-            s = scale_code<FMT>(amax);
-            const float up = scale_up(s);
-            constexpr int kWords = FMT == S24_MXFP4 ? 1 : 2;
-            uint32_t code[kWords], other[kWords];
-            encode8<FMT>(y, exact ? up : up * (1.0f - 0x1p-21f), code);
-            encode8<FMT>(y, exact ? up : up * (1.0f + 0x1p-21f), other);
-            bool differ = code[0] != other[0];
-            if (kWords == 2) differ = differ || code[kWords - 1] != other[kWords - 1];
-            if (differ && s != 255u) {
-                norm_exact<DT>(h[c], w, rhi, rlo, y);
-                encode8<FMT>(y, up, code);
-            }
-            if (s == 255u) {
+        for (int i = 0; i < 8; ++i) w[i] = 0u;
+        if (ok) load32(p.weight + at * 32, w);
+        Pair y[8];
 #pragma unroll
-                for (int i = 0; i < kWords; ++i) code[i] = 0u;
-            }
-            uint8_t* dst = p.codes + (int64_t)r * p.KB * Format<FMT>::kBytes;
-            if constexpr (FMT == S24_MXFP4) reinterpret_cast<uint32_t*>(dst)[at] = code[0];
-            else reinterpret_cast<uint2*>(dst)[at] = make_uint2(code[0], code[1]);
-            if (p.scales != nullptr && (threadIdx.x & 3) == 0) p.scales[(int64_t)r * p.KB + kb] = (uint8_t)s;
+        for (int i = 0; i < 8; ++i) {
+            const float2 a = unpack2<DT>(h[c][i]), b = unpack2<DT>(w[i]);
+            y[i] = make_pair(a.x, a.y) * make_pair(rhi, rhi) * make_pair(b.x, b.y);
         }
-        if (p.scales_tc != nullptr && (threadIdx.x & 3) == 0 && r < p.R_pad && kb < p.KB_pad)
-            p.scales_tc[tc_offset(r, kb, p.KB_pad >> 2)] = (uint8_t)s;
+        float m = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float2 f = split(y[i]);
+            m = max_magnitude(m, f.x, f.y);
+        }
+        uint32_t amax = __float_as_uint(m);   // a NaN among them gives a NaN's bits, the largest
+        amax = max(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 1));
+        const uint8_t* h_at = (p.residual != nullptr ? p.h + (int64_t)r * (p.KB * 64) : p.x + (int64_t)r * p.x_row_bytes) + at * 32;
+        const uint8_t* w_at = p.weight + at * 32;
+        // a power of two too near to tell the scale, or numbers too small for fp32's own rounding
+        const bool unsure = ((amax + 8u) & 0x7FFFFFu) < 16u || amax - 1u < 0x0E800000u;
+        if (__any_sync(0xFFFFFFFFu, unsure)) {
+            uint32_t exact = 0;
+            if (ok) {
+#pragma unroll 1
+                for (int e = 0; e < 16; ++e) exact = max(exact, magnitude_bits(norm_exact<DT>(h_at + 2 * e, w_at + 2 * e, rhi, rlo)));
+            }
+            exact = max(exact, __shfl_xor_sync(0xFFFFFFFFu, exact, 1));
+            if (unsure) amax = exact;
+        }
+        const uint32_t s = scale_code<FMT>(amax);
+        const float up = scale_up(s);
+        constexpr int kWords = FMT == S24_MXFP4 ? 2 : 4, kBits = FMT == S24_MXFP4 ? 4 : 8;
+        uint32_t code[kWords], other[kWords];
+        encode_piece<FMT>(y, up * (1.0f - 0x1p-21f), code);
+        encode_piece<FMT>(y, up * (1.0f + 0x1p-21f), other);
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) {
+            uint32_t d = ok ? (unsure ? 0xFFFFFFFFu : code[i] ^ other[i]) : 0u;
+#pragma unroll 1
+            while (d != 0u) {   // an element that the two do not agree on
+                const int e = (__ffs((int)d) - 1) / kBits;
+                const uint32_t mask = ((1u << kBits) - 1u) << (e * kBits);
+                const int at_e = 2 * (i * (32 / kBits) + e);
+                float one[8] = {norm_exact<DT>(h_at + at_e, w_at + at_e, rhi, rlo) * up, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+                const uint32_t q = FMT == S24_MXFP4 ? to_e2m1x8(one) : to_e4m3x4(one);
+                code[i] = (code[i] & ~mask) | ((q << (e * kBits)) & mask);
+                d &= ~mask;
+            }
+        }
+        if (s == 255u) {
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) code[i] = 0u;
+        }
+        if (ok) {
+            if constexpr (FMT == S24_MXFP4) *reinterpret_cast<uint2*>(codes + at * 8) = make_uint2(code[0], code[1]);
+            else *reinterpret_cast<uint4*>(codes + at * 16) = make_uint4(code[0], code[1], code[2], code[3]);
+            if (p.scales != nullptr && (threadIdx.x & 1) == 0) p.scales[(int64_t)r * p.KB + kb] = (uint8_t)s;
+        }
+        if (p.scales_tc != nullptr && (threadIdx.x & 1) == 0 && r < p.R_pad && kb < p.KB_pad)
+            p.scales_tc[tc_offset(r, kb, p.KB_pad >> 2)] = ok ? (uint8_t)s : (uint8_t)0;
     }
 }
 
 template <int DT, int FMT, int TPR, int NC>
-static int launch_norm(const NormParams& p, cudaStream_t st)
+static int launch_norm(const NormParams& p, int threads, cudaStream_t st)
 {
-    constexpr int kThreads = TPR < 128 ? 128 : TPR;
-    constexpr uint32_t kRows = kThreads / TPR;
-    mx_rms_norm_kernel<DT, FMT, TPR, NC><<<(p.R_pad + kRows - 1) / kRows, kThreads, 0, st>>>(p);
+    const uint32_t rows = TPR == 0 ? 1 : 128 / (TPR == 0 ? 1 : TPR);
+    mx_rms_norm_kernel<DT, FMT, TPR, NC><<<(p.R_pad + rows - 1) / rows, threads, 0, st>>>(p);
     return check_cuda(cudaGetLastError(), "mx_rms_norm launch");
 }
 
-// Four pieces of eight elements per thread, a block's worth, wherever the row allows it: the smallest power of two of
-// threads that covers the row; beyond 512 threads, 8 or 16 pieces per thread.
+// Two pieces of 16 elements per thread: rows of at most 1024 share a CTA, longer ones have as many warps as it takes, and
+// beyond 32768 elements the 1024 threads take four pieces each.
 template <int DT, int FMT>
 static int pick_norm(const NormParams& p, cudaStream_t st)
 {
-    const uint32_t kb = p.KB_pad;
-    if (kb <= 4) return launch_norm<DT, FMT, 4, 4>(p, st);
-    if (kb <= 8) return launch_norm<DT, FMT, 8, 4>(p, st);
-    if (kb <= 16) return launch_norm<DT, FMT, 16, 4>(p, st);
-    if (kb <= 32) return launch_norm<DT, FMT, 32, 4>(p, st);
-    if (kb <= 64) return launch_norm<DT, FMT, 64, 4>(p, st);
-    if (kb <= 128) return launch_norm<DT, FMT, 128, 4>(p, st);
-    if (kb <= 256) return launch_norm<DT, FMT, 256, 4>(p, st);
-    if (kb <= 512) return launch_norm<DT, FMT, 512, 4>(p, st);
-    if (kb <= 1024) return launch_norm<DT, FMT, 512, 8>(p, st);
-    return launch_norm<DT, FMT, 512, 16>(p, st);
+    const int threads = (int)((p.KB_pad + 31) / 32 * 32);   // KB_pad blocks are 2 KB_pad pieces
+    if (threads > 1024) return launch_norm<DT, FMT, 0, 4>(p, 1024, st);
+    if (threads > 32) return launch_norm<DT, FMT, 0, 2>(p, threads, st);
+    if (p.KB_pad > 16) return launch_norm<DT, FMT, 32, 2>(p, 128, st);
+    if (p.KB_pad > 8) return launch_norm<DT, FMT, 16, 2>(p, 128, st);
+    if (p.KB_pad > 4) return launch_norm<DT, FMT, 8, 2>(p, 128, st);
+    return launch_norm<DT, FMT, 4, 2>(p, 128, st);
 }
 
 }  // namespace s24
@@ -271,10 +265,11 @@ extern "C" int s24_mx_rms_norm(const void* x, const void* residual, const void* 
     if (R == 0 || K == 0) return S24_OK;
     if (x == nullptr || weight == nullptr || codes == nullptr || (scales == nullptr && scales_tc == nullptr) || (residual != nullptr && h == nullptr))
         return fail(S24_ERR_INVALID_ARG, "mx_rms_norm: null pointer");
-    if (ldx < K || ldx > (INT64_MAX >> 2) / R || ldx % 8 != 0 || (residual != nullptr && (ldr < K || ldr > (INT64_MAX >> 2) / R || ldr % 8 != 0)))
-        return fail(S24_ERR_SHAPE, "mx_rms_norm: row strides must be >= K and multiples of 8 (got %lld, %lld)", (long long)ldx, (long long)ldr);
-    if (!aligned(x, 16) || !aligned(residual, 16) || !aligned(weight, 16) || !aligned(h, 16) || !aligned(codes, 16) || !aligned(scales_tc, 16))
-        return fail(S24_ERR_INVALID_ARG, "mx_rms_norm: pointers must be 16-byte aligned");
+    if (ldx < K || ldx > (INT64_MAX >> 2) / R || ldx % 16 != 0 || (residual != nullptr && (ldr < K || ldr > (INT64_MAX >> 2) / R || ldr % 16 != 0)))
+        return fail(S24_ERR_SHAPE, "mx_rms_norm: row strides must be >= K and multiples of 16 (got %lld, %lld)", (long long)ldx, (long long)ldr);
+    if (!aligned(x, 32) || !aligned(residual, 32) || !aligned(weight, 32) || (residual != nullptr && !aligned(h, 32)) || !aligned(codes, 16) ||
+        !aligned(scales_tc, 16))
+        return fail(S24_ERR_INVALID_ARG, "mx_rms_norm: x, residual, weight and h must be 32-byte aligned, codes and scales_tc 16");
     NormParams p;
     p.x = static_cast<const uint8_t*>(x);
     p.residual = static_cast<const uint8_t*>(residual);

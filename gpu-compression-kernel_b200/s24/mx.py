@@ -193,9 +193,9 @@ def mx_rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residu
     codes, scales, tc = _new_quantized(x.shape[:-1], R, K, f, want_rows, want_tc, x.device)
     h = x if residual is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
     if R * K:
-        m, ldx = _matrix(x, R, 16)
-        r, ldr = (None, 0) if residual is None else _matrix(residual, R, 16)
-        w, _ = _matrix(weight, 1, 16)
+        m, ldx = _matrix(x, R, 32)
+        r, ldr = (None, 0) if residual is None else _matrix(residual, R, 32)
+        w = weight if weight.stride(0) == 1 and weight.data_ptr() % 32 == 0 else weight.clone(memory_format=torch.contiguous_format)
         _call("s24_mx_rms_norm", x, d, m.data_ptr(), _ptr(r), w.data_ptr(), None if residual is None else h.data_ptr(), R, K, ldx, ldr, eps,
               _DT[x.dtype], f, codes.data_ptr(), _ptr(scales), _ptr(tc))
     return codes, scales, tc, h
