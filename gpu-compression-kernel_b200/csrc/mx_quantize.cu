@@ -8,11 +8,27 @@ using namespace mx;
 
 constexpr int kQuantThreads = 256;
 
-__device__ __forceinline__ uint4 load16(const void* p)
+// scale code and codes of a block
+template <int FMT>
+__device__ __forceinline__ uint32_t quantize_block(const Pair (&v)[kBlock / 2], uint32_t (&c)[Format<FMT>::kBytes / 4])
 {
-    uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-    return v;
+    float m = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kBlock / 2; ++i) {
+        const float2 f = split(v[i]);
+        m = max_magnitude(m, f.x, f.y);
+    }
+    const uint32_t s = scale_code<FMT>(__float_as_uint(m));   // a NaN among them gives a NaN's bits
+    const float up = scale_up(s);
+    float u[kBlock];
+#pragma unroll
+    for (int i = 0; i < kBlock / 2; ++i) {
+        const float2 f = split(v[i] * make_pair(up, up));
+        u[2 * i] = f.x;
+        u[2 * i + 1] = f.y;
+    }
+    encode_block<FMT>(u, s != 255u, c);
+    return s;
 }
 
 // One thread per block of 32 elements; four neighbouring threads share a 128-column chunk and put its
@@ -29,35 +45,26 @@ mx_quantize_kernel(const uint8_t* __restrict__ x, uint32_t R, uint32_t KB, uint3
     uint32_t s = 0;
     if (t < total && r < R && kb < KB) {
         const uint8_t* src = x + (int64_t)r * row_bytes + (int64_t)kb * (kBlock * kElem);
-        float v[kBlock];
+        Pair v[kBlock / 2];
 #pragma unroll
-        for (int i = 0; i < 2 * kElem; ++i) {
-            const uint4 w = load16(src + 16 * i);
-            const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+        for (int i = 0; i < kElem; ++i) {
+            uint32_t u[8];
+            load32(src + 32 * i, u);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
+            for (int j = 0; j < 8; ++j) {
                 if constexpr (DT == S24_FP32) {
-                    v[4 * i + j] = __uint_as_float(u[j]);
+                    if (j & 1) v[4 * i + j / 2] = make_pair(__uint_as_float(u[j - 1]), __uint_as_float(u[j]));
                 } else {
                     const float2 f = unpack2<DT>(u[j]);
-                    v[8 * i + 2 * j] = f.x;
-                    v[8 * i + 2 * j + 1] = f.y;
+                    v[8 * i + j] = make_pair(f.x, f.y);
                 }
             }
         }
-        uint32_t amax = 0;
-#pragma unroll
-        for (int i = 0; i < kBlock; ++i) amax = max(amax, magnitude_bits(v[i]));
-        s = scale_code<FMT>(amax);
-        const float up = scale_up(s);
-#pragma unroll
-        for (int i = 0; i < kBlock; ++i) v[i] *= up;
         uint32_t c[Format<FMT>::kBytes / 4];
-        encode_block<FMT>(v, s != 255u, c);
+        s = quantize_block<FMT>(v, c);
         const int64_t at = (int64_t)r * KB + kb;
-        uint4* dst = reinterpret_cast<uint4*>(codes + at * Format<FMT>::kBytes);
-#pragma unroll
-        for (int i = 0; i < Format<FMT>::kBytes / 16; ++i) dst[i] = make_uint4(c[4 * i], c[4 * i + 1], c[4 * i + 2], c[4 * i + 3]);
+        if constexpr (FMT == S24_MXFP4) *reinterpret_cast<uint4*>(codes + at * 16) = make_uint4(c[0], c[1], c[2], c[3]);
+        else store32(codes + at * 32, c);
         if (scales != nullptr) scales[at] = (uint8_t)s;
     }
     if constexpr (TC) {
@@ -80,32 +87,35 @@ mx_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restric
     const uint32_t r = t / KB, kb = t - r * KB;
     const float s = scale_value(scales[tc ? tc_offset(r, kb, (KB + 3) / 4) : (int64_t)t]);
     const uint8_t* src = codes + (int64_t)t * Format<FMT>::kBytes;
-    float v[kBlock];
+    uint32_t u[Format<FMT>::kBytes / 4];
+    if constexpr (FMT == S24_MXFP4) {
+        const uint4 w = *reinterpret_cast<const uint4*>(src);
+        u[0] = w.x; u[1] = w.y; u[2] = w.z; u[3] = w.w;
+    } else {
+        load32(src, u);
+    }
+    uint8_t* dst = out + (int64_t)t * (kBlock * kElem);
+    constexpr int kPer = 32 / kElem;   // elements of a 32-byte store
 #pragma unroll
-    for (int i = 0; i < Format<FMT>::kBytes / 16; ++i) {
-        const uint4 w = load16(src + 16 * i);
-        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+    for (int i = 0; i < kElem; ++i) {
+        float v[kPer];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < kPer; j += 4) {
+            const int e = kPer * i + j;
             if constexpr (FMT == S24_MXFP4) {
-                from_e2m1x4(u[j] & 0xFFFFu, &v[8 * j]);
-                from_e2m1x4(u[j] >> 16, &v[8 * j + 4]);
+                from_e2m1x4((u[e / 8] >> (4 * (e & 7))) & 0xFFFFu, &v[j]);
             } else {
-                from_e4m3x2(u[j] & 0xFFFFu, &v[16 * i + 4 * j]);
-                from_e4m3x2(u[j] >> 16, &v[16 * i + 4 * j + 2]);
+                from_e4m3x2(u[e / 4] & 0xFFFFu, &v[j]);
+                from_e4m3x2(u[e / 4] >> 16, &v[j + 2]);
             }
         }
-    }
-    uint4* dst = reinterpret_cast<uint4*>(out + (int64_t)t * (kBlock * kElem));
+        uint32_t q[8];
 #pragma unroll
-    for (int i = 0; i < 2 * kElem; ++i) {
-        uint32_t u[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if constexpr (DT == S24_FP32) u[j] = __float_as_uint(v[4 * i + j] * s);
-            else u[j] = mx::pack2<DT>(v[8 * i + 2 * j] * s, v[8 * i + 2 * j + 1] * s);
+        for (int j = 0; j < 8; ++j) {
+            if constexpr (DT == S24_FP32) q[j] = __float_as_uint(v[j] * s);
+            else q[j] = mx::pack2<DT>(v[2 * j] * s, v[2 * j + 1] * s);
         }
-        dst[i] = make_uint4(u[0], u[1], u[2], u[3]);
+        store32(dst + 32 * i, q);
     }
 }
 
@@ -182,10 +192,10 @@ extern "C" int s24_mx_quantize(const void* x, int64_t R, int64_t K, int64_t ld, 
     if (x == nullptr || codes == nullptr || (scales == nullptr && scales_tc == nullptr))
         return fail(S24_ERR_INVALID_ARG, "mx_quantize: null pointer");
     const int64_t elem = dtype == S24_FP32 ? 4 : 2;
-    if (ld < K || ld > (INT64_MAX >> 2) / R || (ld * elem) % 16 != 0)
-        return fail(S24_ERR_SHAPE, "mx_quantize: the row stride must be >= K and a multiple of 16 bytes (got %lld elements)", (long long)ld);
-    if (!aligned(x, 16) || !aligned(codes, 16) || !aligned(scales_tc, 16))
-        return fail(S24_ERR_INVALID_ARG, "mx_quantize: pointers must be 16-byte aligned");
+    if (ld < K || ld > (INT64_MAX >> 2) / R || (ld * elem) % 32 != 0)
+        return fail(S24_ERR_SHAPE, "mx_quantize: the row stride must be >= K and a multiple of 32 bytes (got %lld elements)", (long long)ld);
+    if (!aligned(x, 32) || !aligned(codes, 32) || !aligned(scales_tc, 16))
+        return fail(S24_ERR_INVALID_ARG, "mx_quantize: x and codes must be 32-byte aligned, scales_tc 16");
     auto st = static_cast<cudaStream_t>(stream);
     if (fmt == S24_MXFP4) {
         if (dtype == S24_FP16) launch_quantize<S24_FP16, S24_MXFP4>(x, R, K, ld * elem, codes, scales, scales_tc, st);
@@ -209,7 +219,7 @@ extern "C" int s24_mx_dequantize(const void* codes, const void* scales, int layo
     if (rc) return rc;
     if (R == 0 || K == 0) return S24_OK;
     if (codes == nullptr || scales == nullptr || out == nullptr) return fail(S24_ERR_INVALID_ARG, "mx_dequantize: null pointer");
-    if (!aligned(codes, 16) || !aligned(out, 16)) return fail(S24_ERR_INVALID_ARG, "mx_dequantize: pointers must be 16-byte aligned");
+    if (!aligned(codes, 32) || !aligned(out, 32)) return fail(S24_ERR_INVALID_ARG, "mx_dequantize: codes and out must be 32-byte aligned");
     auto st = static_cast<cudaStream_t>(stream);
     if (fmt == S24_MXFP4) {
         if (dtype == S24_FP16) launch_dequantize<S24_FP16, S24_MXFP4>(codes, scales, layout, out, R, K, st);

@@ -137,7 +137,7 @@ def mx_quantize(x: torch.Tensor, fmt: str = "mxfp4", want_rows: bool = True, wan
     d = _device_of(x)
     codes, scales, tc = _new_quantized(x.shape[:-1], R, K, f, want_rows, want_tc, x.device)
     if R * K:
-        m, ld = _matrix(x, R, 16)
+        m, ld = _matrix(x, R, 32)
         _call("s24_mx_quantize", x, d, m.data_ptr(), R, K, ld, _DT[x.dtype], f, codes.data_ptr(), _ptr(scales), _ptr(tc))
     return codes, scales, tc
 
@@ -151,7 +151,7 @@ def mx_dequantize(codes: torch.Tensor, scales: torch.Tensor, layout: str = "rows
     d = _device_of(codes, scales)
     out = torch.empty((*codes.shape[:-1], K), dtype=dtype, device=codes.device)
     if R * K:
-        c = codes if codes.is_contiguous() and codes.data_ptr() % 16 == 0 else codes.clone(memory_format=torch.contiguous_format)
+        c = codes if codes.is_contiguous() and codes.data_ptr() % 32 == 0 else codes.clone(memory_format=torch.contiguous_format)
         _call("s24_mx_dequantize", codes, d, c.data_ptr(), scales.data_ptr(), _SCALES[layout], out.data_ptr(), R, K, f, _DT[dtype])
     return out
 

@@ -307,14 +307,14 @@ S24_API size_t s24_mx_scales_tc_bytes(int64_t R, int64_t K);
 /*
  * Quantise x (R, K; row stride ld elements; S24_FP16, S24_BF16 or S24_FP32) to `fmt` in one pass: codes
  * (contiguous) and the scales in either layout or both (one of the two pointers may be NULL).
- * K % 32 == 0, row stride a multiple of 16 bytes; x, codes and scales_tc 16-byte aligned.  R = 0 or
+ * K % 32 == 0, row stride a multiple of 32 bytes; x and codes 32-byte aligned, scales_tc 16.  R = 0 or
  * K = 0 does nothing.
  */
 S24_API int s24_mx_quantize(const void* x, int64_t R, int64_t K, int64_t ld, int dtype, int fmt,
                     void* codes, void* scales, void* scales_tc, void* stream);
 
 /* Read codes and scales (in `layout`) back: out (R, K) contiguous, S24_FP16, S24_BF16 or S24_FP32, rounded once.
- * codes and out 16-byte aligned, K % 32 == 0. */
+ * codes and out 32-byte aligned, K % 32 == 0. */
 S24_API int s24_mx_dequantize(const void* codes, const void* scales, int layout, void* out, int64_t R, int64_t K,
                       int fmt, int dtype, void* stream);
 
