@@ -91,13 +91,14 @@ def _check_k(k: int) -> None:
         raise RuntimeError(f"the last dimension must be divisible by 32, the size of a block (got {k})")
 
 
-def _new_quantized(lead, R: int, K: int, fmt: int, want_rows: bool, want_tc: bool, device):
+def _new_quantized(x: torch.Tensor, R: int, K: int, fmt: int, want_rows: bool, want_tc: bool):
     if not want_rows and not want_tc:
         raise RuntimeError("ask for at least one layout of the scales (want_rows, want_tc)")
-    codes = (torch.empty((*lead, K // 2), dtype=torch.uint8, device=device) if fmt == L.MXFP4
-             else torch.empty((*lead, K), dtype=torch.float8_e4m3fn, device=device))
-    scales = torch.empty((*lead, K // 32), dtype=torch.uint8, device=device) if want_rows else None
-    tc = torch.empty((mx_scales_numel(R, K),), dtype=torch.uint8, device=device) if want_tc else None
+    lead = x.shape[:-1]
+    codes = (x.new_empty((*lead, K // 2), dtype=torch.uint8) if fmt == L.MXFP4
+             else x.new_empty((*lead, K), dtype=torch.float8_e4m3fn))
+    scales = x.new_empty((*lead, K // 32), dtype=torch.uint8) if want_rows else None
+    tc = x.new_empty((mx_scales_numel(R, K),), dtype=torch.uint8) if want_tc else None
     return codes, scales, tc
 
 
@@ -135,7 +136,7 @@ def mx_quantize(x: torch.Tensor, fmt: str = "mxfp4", want_rows: bool = True, wan
         raise RuntimeError(f"Invalid datatype {x.dtype} of dense matrix")
     _check_k(K)
     d = _device_of(x)
-    codes, scales, tc = _new_quantized(x.shape[:-1], R, K, f, want_rows, want_tc, x.device)
+    codes, scales, tc = _new_quantized(x, R, K, f, want_rows, want_tc)
     if R * K:
         m, ld = _matrix(x, R, 32)
         _call("s24_mx_quantize", x, d, m.data_ptr(), R, K, ld, _DT[x.dtype], f, codes.data_ptr(), _ptr(scales), _ptr(tc))
@@ -149,7 +150,7 @@ def mx_dequantize(codes: torch.Tensor, scales: torch.Tensor, layout: str = "rows
         raise RuntimeError(f"Invalid datatype {dtype} of dense matrix")
     _check_scales(scales, layout, R, K)
     d = _device_of(codes, scales)
-    out = torch.empty((*codes.shape[:-1], K), dtype=dtype, device=codes.device)
+    out = codes.new_empty((*codes.shape[:-1], K), dtype=dtype)
     if R * K:
         c = codes if codes.is_contiguous() and codes.data_ptr() % 32 == 0 else codes.clone(memory_format=torch.contiguous_format)
         _call("s24_mx_dequantize", codes, d, c.data_ptr(), scales.data_ptr(), _SCALES[layout], out.data_ptr(), R, K, f, _DT[dtype])
@@ -164,7 +165,7 @@ def mx_scales_convert(scales: torch.Tensor, from_layout: str, to_layout: str, R:
         raise ValueError(f"cannot convert scales from {from_layout!r} to {to_layout!r}")
     d = _device_of(scales)
     shape = (R, K // 32) if to_layout == "rows" else (mx_scales_numel(R, K),)
-    out = torch.empty(shape, dtype=torch.uint8, device=scales.device)
+    out = scales.new_empty(shape, dtype=torch.uint8)
     if R * K:
         _call("s24_mx_scales_convert", scales, d, scales.data_ptr(), _SCALES[from_layout], out.data_ptr(), _SCALES[to_layout], R, K)
     return out
@@ -190,8 +191,8 @@ def mx_rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residu
     if K > L.MX_NORM_MAX_K:
         raise RuntimeError(f"rows of at most {L.MX_NORM_MAX_K} elements (got {K})")
     d = _device_of(x, weight, residual)
-    codes, scales, tc = _new_quantized(x.shape[:-1], R, K, f, want_rows, want_tc, x.device)
-    h = x if residual is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    codes, scales, tc = _new_quantized(x, R, K, f, want_rows, want_tc)
+    h = x if residual is None else torch.empty_like(x, memory_format=torch.contiguous_format)
     if R * K:
         m, ldx = _matrix(x, R, 32)
         r, ldr = (None, 0) if residual is None else _matrix(residual, R, 32)
@@ -223,7 +224,7 @@ def mx_matmul(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_scales
     _check_scales(b_scales, "tc", N, K)
     d = _device_of(a, a_scales, b, b_scales, out)
     if out is None:
-        c = torch.empty((*a.shape[:-1], N), dtype=out_dtype, device=a.device)
+        c = a.new_empty((*a.shape[:-1], N), dtype=out_dtype)
         ldc = N
     else:
         c = out
