@@ -141,6 +141,33 @@ __device__ __forceinline__ uint32_t pack2(float a, float b)
     }
 }
 
+// Launches that follow one another overlap: a kernel lets the next one of its stream start as soon as all its own CTAs have
+// (start_dependents), and touches global memory only when the kernels before it have completed and their writes are visible
+// (wait_for_predecessors).  What it does before that, setting up barriers, tensor memory and descriptors, costs nothing then.
+// A kernel of another library neither starts early nor is overtaken.
+__device__ __forceinline__ void start_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_predecessors() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+template <class... Params, class... Args>
+inline cudaError_t launch_overlapped(void (*kernel)(Params...), dim3 grid, unsigned threads, size_t smem, unsigned cluster, cudaStream_t stream, Args... args)
+{
+    cudaLaunchConfig_t lc = {};
+    lc.gridDim = grid;
+    lc.blockDim = dim3(threads);
+    lc.dynamicSmemBytes = smem;
+    lc.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    lc.attrs = attr;
+    lc.numAttrs = cluster > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&lc, kernel, args...);
+}
+
 // two fp32 numbers in one 64-bit register pair, and operations on both at once
 struct Pair {
     uint64_t v;

@@ -258,6 +258,8 @@ mx_matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
     if (G == 2) cluster_sync();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot_ptr;
+    mx::start_dependents();
+    mx::wait_for_predecessors();
 
     if (warp == 0) {
         // ------------------------------------------------------------ TMA producer
@@ -526,6 +528,8 @@ mx_matmul_few_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot_ptr;
+    mx::start_dependents();
+    mx::wait_for_predecessors();
 
     if (warp == 0) {
         if (elect_one()) {
@@ -681,19 +685,9 @@ static int launch_mx(const MxOperand& a, const MxOperand& b, MxParams p, cudaStr
     if (tiles > 0x7FFFFFFFll / kGroupM) return fail(S24_ERR_SHAPE, "mx_matmul: too many output tiles");
     int units = sm_count() / Cfg::kG;
     if (units > tiles) units = (int)tiles;
-    cudaLaunchConfig_t lc = {};
-    lc.gridDim = dim3((unsigned)(units * Cfg::kG));
-    lc.blockDim = dim3(kMxThreads);
-    lc.dynamicSmemBytes = Cfg::kSmemBytes;
-    lc.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = Cfg::kG;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    lc.attrs = attr;
-    lc.numAttrs = 1;
-    return check_cuda(cudaLaunchKernelEx(&lc, mx_matmul_kernel<Cfg>, tm_a, tm_b, tm_sa, tm_sb, p), "mx_matmul launch");
+    return check_cuda(mx::launch_overlapped(mx_matmul_kernel<Cfg>, dim3((unsigned)(units * Cfg::kG)), kMxThreads, Cfg::kSmemBytes, Cfg::kG, stream, tm_a, tm_b,
+                                            tm_sa, tm_sb, p),
+                      "mx_matmul launch");
 }
 
 // K split of the kernel for few rows: as many CTAs as find room at once (two per SM), but a second CTA on an SM only
@@ -734,19 +728,9 @@ static int launch_few(const MxOperand& a, const MxOperand& b, FewParams p, int64
     const int tiles = (p.n_long + 127) / 128;
     if (split == 0) split = few_split(tiles, p.ktiles);
     if (split > p.ktiles) split = 1;
-    cudaLaunchConfig_t lc = {};
-    lc.gridDim = dim3((unsigned)split, (unsigned)tiles);
-    lc.blockDim = dim3(kFewThreads);
-    lc.dynamicSmemBytes = Cfg::kSmemBytes;
-    lc.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)split;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    lc.attrs = attr;
-    lc.numAttrs = 1;
-    return check_cuda(cudaLaunchKernelEx(&lc, mx_matmul_few_kernel<Cfg>, tm_a, tm_b, tm_sa, tm_sb, p), "mx_matmul launch");
+    return check_cuda(mx::launch_overlapped(mx_matmul_few_kernel<Cfg>, dim3((unsigned)split, (unsigned)tiles), kFewThreads, Cfg::kSmemBytes, (unsigned)split, stream,
+                                            tm_a, tm_b, tm_sa, tm_sb, p),
+                      "mx_matmul launch");
 }
 
 template <bool F4>

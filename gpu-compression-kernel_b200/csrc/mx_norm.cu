@@ -101,6 +101,7 @@ mx_rms_norm_kernel(const NormParams p)
     const uint32_t r = TPR == 0 ? blockIdx.x : blockIdx.x * (128 / (TPR == 0 ? 1 : TPR)) + threadIdx.x / (TPR == 0 ? 1 : TPR);
     const uint32_t pieces = r < p.R ? p.KB * 2 : 0;
 
+    wait_for_predecessors();   // and no early start of the next kernel: its CTAs would share the issue slots that this one lives on
     uint32_t h[NC][8];
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
@@ -230,8 +231,7 @@ template <int DT, int FMT, int TPR, int NC>
 static int launch_norm(const NormParams& p, int threads, cudaStream_t st)
 {
     const uint32_t rows = TPR == 0 ? 1 : 128 / (TPR == 0 ? 1 : TPR);
-    mx_rms_norm_kernel<DT, FMT, TPR, NC><<<(p.R_pad + rows - 1) / rows, threads, 0, st>>>(p);
-    return check_cuda(cudaGetLastError(), "mx_rms_norm launch");
+    return check_cuda(launch_overlapped(mx_rms_norm_kernel<DT, FMT, TPR, NC>, dim3((p.R_pad + rows - 1) / rows), (unsigned)threads, 0, 1, st, p), "mx_rms_norm launch");
 }
 
 // Two pieces of 16 elements per thread: rows of at most 1024 share a CTA, longer ones have as many warps as it takes, and

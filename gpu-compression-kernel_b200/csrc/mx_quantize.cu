@@ -43,6 +43,8 @@ mx_quantize_kernel(const uint8_t* __restrict__ x, uint32_t R, uint32_t KB, uint3
     const uint32_t t = blockIdx.x * kQuantThreads + threadIdx.x;
     const uint32_t r = t / KB_pad, kb = t - r * KB_pad;
     uint32_t s = 0;
+    start_dependents();
+    wait_for_predecessors();
     if (t < total && r < R && kb < KB) {
         const uint8_t* src = x + (int64_t)r * row_bytes + (int64_t)kb * (kBlock * kElem);
         Pair v[kBlock / 2];
@@ -83,6 +85,8 @@ mx_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restric
 {
     constexpr int kElem = DT == S24_FP32 ? 4 : 2;
     const uint32_t t = blockIdx.x * kQuantThreads + threadIdx.x;
+    start_dependents();
+    wait_for_predecessors();
     if (t >= total) return;
     const uint32_t r = t / KB, kb = t - r * KB;
     const float s = scale_value(scales[tc ? tc_offset(r, kb, (KB + 3) / 4) : (int64_t)t]);
@@ -125,6 +129,8 @@ __global__ void __launch_bounds__(kQuantThreads)
 mx_scales_convert_kernel(const uint8_t* __restrict__ src, uint8_t* __restrict__ dst, uint32_t R, uint32_t KB, uint32_t total)
 {
     const uint32_t t = blockIdx.x * kQuantThreads + threadIdx.x;
+    start_dependents();
+    wait_for_predecessors();
     if (t >= total) return;
     const uint32_t chunks = (KB + 3) / 4;
     if constexpr (TO_TC) {
@@ -149,7 +155,7 @@ static int check_mx_shape(const char* who, int64_t R, int64_t K)
 }
 
 template <int DT, int FMT>
-static void launch_quantize(const void* x, int64_t R, int64_t K, int64_t row_bytes, void* codes, void* scales, void* tc, cudaStream_t st)
+static int launch_quantize(const void* x, int64_t R, int64_t K, int64_t row_bytes, void* codes, void* scales, void* tc, cudaStream_t st)
 {
     const uint32_t KB = (uint32_t)(K / kBlock);
     const uint32_t KB_pad = tc ? (uint32_t)(k_chunks(K) * 4) : KB;
@@ -159,16 +165,19 @@ static void launch_quantize(const void* x, int64_t R, int64_t K, int64_t row_byt
     auto* c = static_cast<uint8_t*>(codes);
     auto* s = static_cast<uint8_t*>(scales);
     auto* t = static_cast<uint8_t*>(tc);
-    if (tc) mx_quantize_kernel<DT, FMT, true><<<grid, kQuantThreads, 0, st>>>(xs, (uint32_t)R, KB, KB_pad, total, row_bytes, c, s, t);
-    else mx_quantize_kernel<DT, FMT, false><<<grid, kQuantThreads, 0, st>>>(xs, (uint32_t)R, KB, KB_pad, total, row_bytes, c, s, t);
+    return check_cuda(launch_overlapped(tc ? mx_quantize_kernel<DT, FMT, true> : mx_quantize_kernel<DT, FMT, false>, dim3(grid), kQuantThreads, 0, 1, st,
+                                        xs, (uint32_t)R, KB, KB_pad, total, row_bytes, c, s, t),
+                      "mx_quantize launch");
 }
 
 template <int DT, int FMT>
-static void launch_dequantize(const void* codes, const void* scales, int layout, void* out, int64_t R, int64_t K, cudaStream_t st)
+static int launch_dequantize(const void* codes, const void* scales, int layout, void* out, int64_t R, int64_t K, cudaStream_t st)
 {
     const uint32_t KB = (uint32_t)(K / kBlock), total = (uint32_t)R * KB;
-    mx_dequantize_kernel<DT, FMT><<<(total + kQuantThreads - 1) / kQuantThreads, kQuantThreads, 0, st>>>(
-        static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), layout == S24_SCALES_TC, KB, total, static_cast<uint8_t*>(out));
+    return check_cuda(launch_overlapped(mx_dequantize_kernel<DT, FMT>, dim3((total + kQuantThreads - 1) / kQuantThreads), kQuantThreads, 0, 1, st,
+                                        static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), (int)(layout == S24_SCALES_TC), KB, total,
+                                        static_cast<uint8_t*>(out)),
+                      "mx_dequantize launch");
 }
 
 }  // namespace s24
@@ -198,15 +207,13 @@ extern "C" int s24_mx_quantize(const void* x, int64_t R, int64_t K, int64_t ld, 
         return fail(S24_ERR_INVALID_ARG, "mx_quantize: x and codes must be 32-byte aligned, scales_tc 16");
     auto st = static_cast<cudaStream_t>(stream);
     if (fmt == S24_MXFP4) {
-        if (dtype == S24_FP16) launch_quantize<S24_FP16, S24_MXFP4>(x, R, K, ld * elem, codes, scales, scales_tc, st);
-        else if (dtype == S24_BF16) launch_quantize<S24_BF16, S24_MXFP4>(x, R, K, ld * elem, codes, scales, scales_tc, st);
-        else launch_quantize<S24_FP32, S24_MXFP4>(x, R, K, ld * elem, codes, scales, scales_tc, st);
-    } else {
-        if (dtype == S24_FP16) launch_quantize<S24_FP16, S24_MXFP8>(x, R, K, ld * elem, codes, scales, scales_tc, st);
-        else if (dtype == S24_BF16) launch_quantize<S24_BF16, S24_MXFP8>(x, R, K, ld * elem, codes, scales, scales_tc, st);
-        else launch_quantize<S24_FP32, S24_MXFP8>(x, R, K, ld * elem, codes, scales, scales_tc, st);
+        if (dtype == S24_FP16) return launch_quantize<S24_FP16, S24_MXFP4>(x, R, K, ld * elem, codes, scales, scales_tc, st);
+        if (dtype == S24_BF16) return launch_quantize<S24_BF16, S24_MXFP4>(x, R, K, ld * elem, codes, scales, scales_tc, st);
+        return launch_quantize<S24_FP32, S24_MXFP4>(x, R, K, ld * elem, codes, scales, scales_tc, st);
     }
-    return check_cuda(cudaGetLastError(), "mx_quantize launch");
+    if (dtype == S24_FP16) return launch_quantize<S24_FP16, S24_MXFP8>(x, R, K, ld * elem, codes, scales, scales_tc, st);
+    if (dtype == S24_BF16) return launch_quantize<S24_BF16, S24_MXFP8>(x, R, K, ld * elem, codes, scales, scales_tc, st);
+    return launch_quantize<S24_FP32, S24_MXFP8>(x, R, K, ld * elem, codes, scales, scales_tc, st);
 }
 
 extern "C" int s24_mx_dequantize(const void* codes, const void* scales, int layout, void* out, int64_t R, int64_t K, int fmt, int dtype,
@@ -222,15 +229,13 @@ extern "C" int s24_mx_dequantize(const void* codes, const void* scales, int layo
     if (!aligned(codes, 32) || !aligned(out, 32)) return fail(S24_ERR_INVALID_ARG, "mx_dequantize: codes and out must be 32-byte aligned");
     auto st = static_cast<cudaStream_t>(stream);
     if (fmt == S24_MXFP4) {
-        if (dtype == S24_FP16) launch_dequantize<S24_FP16, S24_MXFP4>(codes, scales, layout, out, R, K, st);
-        else if (dtype == S24_BF16) launch_dequantize<S24_BF16, S24_MXFP4>(codes, scales, layout, out, R, K, st);
-        else launch_dequantize<S24_FP32, S24_MXFP4>(codes, scales, layout, out, R, K, st);
-    } else {
-        if (dtype == S24_FP16) launch_dequantize<S24_FP16, S24_MXFP8>(codes, scales, layout, out, R, K, st);
-        else if (dtype == S24_BF16) launch_dequantize<S24_BF16, S24_MXFP8>(codes, scales, layout, out, R, K, st);
-        else launch_dequantize<S24_FP32, S24_MXFP8>(codes, scales, layout, out, R, K, st);
+        if (dtype == S24_FP16) return launch_dequantize<S24_FP16, S24_MXFP4>(codes, scales, layout, out, R, K, st);
+        if (dtype == S24_BF16) return launch_dequantize<S24_BF16, S24_MXFP4>(codes, scales, layout, out, R, K, st);
+        return launch_dequantize<S24_FP32, S24_MXFP4>(codes, scales, layout, out, R, K, st);
     }
-    return check_cuda(cudaGetLastError(), "mx_dequantize launch");
+    if (dtype == S24_FP16) return launch_dequantize<S24_FP16, S24_MXFP8>(codes, scales, layout, out, R, K, st);
+    if (dtype == S24_BF16) return launch_dequantize<S24_BF16, S24_MXFP8>(codes, scales, layout, out, R, K, st);
+    return launch_dequantize<S24_FP32, S24_MXFP8>(codes, scales, layout, out, R, K, st);
 }
 
 extern "C" int s24_mx_scales_convert(const void* src, int from_layout, void* dst, int to_layout, int64_t R, int64_t K, void* stream)
@@ -248,10 +253,12 @@ extern "C" int s24_mx_scales_convert(const void* src, int from_layout, void* dst
     const uint32_t KB = (uint32_t)(K / kBlock);
     if (to_layout == S24_SCALES_TC) {
         const uint32_t total = (uint32_t)s24_mx_scales_tc_bytes(R, K);
-        mx_scales_convert_kernel<true><<<(total + kQuantThreads - 1) / kQuantThreads, kQuantThreads, 0, st>>>(s, d, (uint32_t)R, KB, total);
-    } else {
-        const uint32_t total = (uint32_t)R * KB;
-        mx_scales_convert_kernel<false><<<(total + kQuantThreads - 1) / kQuantThreads, kQuantThreads, 0, st>>>(s, d, (uint32_t)R, KB, total);
+        return check_cuda(launch_overlapped(mx_scales_convert_kernel<true>, dim3((total + kQuantThreads - 1) / kQuantThreads), kQuantThreads, 0, 1, st, s, d,
+                                            (uint32_t)R, KB, total),
+                          "mx_scales_convert launch");
     }
-    return check_cuda(cudaGetLastError(), "mx_scales_convert launch");
+    const uint32_t total = (uint32_t)R * KB;
+    return check_cuda(launch_overlapped(mx_scales_convert_kernel<false>, dim3((total + kQuantThreads - 1) / kQuantThreads), kQuantThreads, 0, 1, st, s, d,
+                                        (uint32_t)R, KB, total),
+                      "mx_scales_convert launch");
 }
