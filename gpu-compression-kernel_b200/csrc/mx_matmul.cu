@@ -103,11 +103,28 @@ struct MxParams {
     unsigned long long wait_limit_ns;
 };
 
-constexpr int kStorePitch = 9;                               // words: 8 of a row and one against bank conflicts
+constexpr int kStorePitch = 33;                              // words: 32 of a row and one against bank conflicts
 constexpr int kStoreWarpBytes = 32 * kStorePitch * 4;
 
-template <int G, int BN, bool F4, int ST>
+// Tile t of the persistent walk: groups of 16 row tiles swept along N.  Of groups of 4 / 8 / 16 / 32, seconds under load:
+// 8192^3 4-bit 210 / 210 / 208 / 207 us, 8-bit 438 / 428 / 421 / 468, 4001 x 28672 x 8192 700 / 689 / 682 / 682,
+// 16384^3 4-bit 1639 / 1577 / 1550 / 1746.
+constexpr int kMxGroupM = 16;
+__device__ __forceinline__ void mx_tile_coords(int t, int num_m, int num_n, int& tm, int& tn)
+{
+    const int group_size = kMxGroupM * num_n;
+    const int group = t / group_size;
+    const int first_m = group * kMxGroupM;
+    const int gm = min(num_m - first_m, kMxGroupM);
+    const int in_group = t - group * group_size;
+    tm = first_m + in_group % gm;
+    tn = in_group / gm;
+}
+
+// ALIGNED: rows of C start on 32 bytes; otherwise a stage of the ring makes room for the stores' staging
+template <int G, int BN, bool F4, int ST, bool ALIGNED>
 struct MxCfg {
+    static constexpr bool kAligned = ALIGNED;
     static constexpr int kG = G;
     static constexpr int kBN = BN;
     static constexpr bool kF4 = F4;
@@ -124,7 +141,7 @@ struct MxCfg {
     static constexpr int kAccStep = BN >= 256 ? 224 : BN;       // first column of the second accumulator
     static constexpr int kScaleCol0 = kAccStep + BN;
     static constexpr int kScaleCols = 4 * kChunks * (1 + kTilesB);
-    static constexpr int kStoreBytes = 8 * kStoreWarpBytes;
+    static constexpr int kStoreBytes = ALIGNED ? 0 : 8 * kStoreWarpBytes;
     static constexpr int kSmemBytes = ST * kStageBytes + kStoreBytes + 1024 + 256;
     static_assert(kScaleCol0 + kScaleCols <= (int)kTmemCols, "tensor memory budget");
     static_assert(kSmemBytes <= 232448, "shared memory budget");
@@ -138,59 +155,87 @@ __device__ __forceinline__ void store_sector(void* p, const uint32_t* q)
                  : "memory");
 }
 
-// 32 rows (one per lane) x 32 accumulator columns to C.  Rows that allow 32-byte stores take them straight from
-// the registers, a whole sector each (8192^3: 199 us against 203 with 16-byte stores); others go through 1 KB of shared memory, so that 8 lanes write 32 bytes
-// of one row instead of every lane its own row in elements.
-__device__ __forceinline__ void mx_store32(const MxParams& p, int row0, int col, const uint32_t (&r)[32], uint32_t staging, int lane)
+__device__ __forceinline__ uint32_t ld_shared_u32(uint32_t addr)
 {
-    if (row0 >= p.M || col >= p.N) return;   // the same for the whole warp
-    const bool f32 = p.out == S24_FP32;
-    uint32_t q[32];
-    if (f32) {
+    uint32_t v;
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    return v;
+}
+
+// 32 rows (one per lane) x 64 accumulator columns to C, whose rows start on 32 bytes: whole sectors straight from the
+// registers, and single elements where N ends inside one.
+__device__ __forceinline__ void mx_store_aligned(const MxParams& p, int row0, int col, const uint32_t (&r)[64], int lane)
+{
+    const int row = row0 + lane;
+    if (row >= p.M) return;
+    if (p.out == S24_FP32) {
+        float* c = static_cast<float*>(p.C) + (int64_t)row * p.ldc + col;
 #pragma unroll
-        for (int i = 0; i < 32; ++i) q[i] = r[i];
-    } else {
+        for (int i = 0; i < 64; i += 8) {
+            if (col + i + 8 <= p.N) {
+                store_sector(c + i, &r[i]);
+            } else {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) q[i] = pack2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]), p.out == S24_BF16);
-    }
-    if (p.wide && col + 32 <= p.N) {
-        const int64_t at = (int64_t)(row0 + lane) * p.ldc + col;
-        if (row0 + lane < p.M) {
-            uint8_t* c = static_cast<uint8_t*>(p.C) + at * (f32 ? 4 : 2);
-#pragma unroll
-            for (int i = 0; i < 2; ++i) store_sector(c + 32 * i, &q[8 * i]);
-            if (f32) {
-#pragma unroll
-                for (int i = 2; i < 4; ++i) store_sector(c + 32 * i, &q[8 * i]);
+                for (int k = 0; k < 8; ++k)
+                    if (col + i + k < p.N) c[i + k] = __uint_as_float(r[i + k]);
             }
         }
         return;
     }
-    const int word = lane & 7;
+    uint16_t* c = static_cast<uint16_t*>(p.C) + (int64_t)row * p.ldc + col;
 #pragma unroll
-    for (int part = 0; part < 4; ++part) {
-        if (part >= 2 && !f32) break;
+    for (int i = 0; i < 64; i += 16) {
+        uint32_t q[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) q[k] = pack2(__uint_as_float(r[i + 2 * k]), __uint_as_float(r[i + 2 * k + 1]), p.out == S24_BF16);
+        if (col + i + 16 <= p.N) {
+            store_sector(c + i, q);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 16; ++k)
+                if (col + i + k < p.N) c[i + k] = (uint16_t)(q[k >> 1] >> (16 * (k & 1)));
+        }
+    }
+}
+
+// The same for rows that start anywhere: through shared memory, so that 32 lanes write 128 bytes of one row.  16-bit rows
+// that start on an odd element are written as words from their second element on.  (32 bytes of four rows at a time took
+// 52.9 us at 1537 x 6150 x 4128, this 50.8; without any stores it is 42.2.)
+__device__ __forceinline__ void mx_store_any(const MxParams& p, int row0, int col, const uint32_t (&r)[64], uint32_t staging, int lane)
+{
+    const bool f32 = p.out == S24_FP32;
+    const int rows = min(32, p.M - row0);   // the same for the whole warp
+#pragma unroll
+    for (int part = 0; part < 2; ++part) {
+        if (part == 1 && !f32) break;
         __syncwarp();
 #pragma unroll
-        for (int i = 0; i < 8; ++i) st_shared_u32(staging + (uint32_t)(lane * kStorePitch + i) * 4, q[8 * part + i]);
+        for (int i = 0; i < 32; ++i) {
+            const uint32_t w = f32 ? r[32 * part + i] : pack2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]), p.out == S24_BF16);
+            st_shared_u32(staging + (uint32_t)(lane * kStorePitch + i) * 4, w);
+        }
         __syncwarp();
-#pragma unroll 4
-        for (int i = 0; i < 8; ++i) {
-            const int rr = 4 * i + (lane >> 3), row = row0 + rr;
-            uint32_t v;
-            asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(staging + (uint32_t)(rr * kStorePitch + word) * 4) : "memory");
-            if (row >= p.M) continue;
-            if (f32) {
-                const int c = col + 8 * part + word;
-                if (c < p.N) static_cast<float*>(p.C)[(int64_t)row * p.ldc + c] = __uint_as_float(v);
-            } else {
-                const int c = col + 2 * (8 * part + word);
-                uint16_t* dst = static_cast<uint16_t*>(p.C) + (int64_t)row * p.ldc + c;
-                if (c + 1 < p.N && (reinterpret_cast<uintptr_t>(dst) & 3u) == 0) {
-                    *reinterpret_cast<uint32_t*>(dst) = v;
+        if (f32) {
+            const int c = col + 32 * part + lane;
+            float* dst = static_cast<float*>(p.C) + (int64_t)row0 * p.ldc + c;
+            if (c < p.N) {
+#pragma unroll 8
+                for (int rr = 0; rr < rows; ++rr, dst += p.ldc) *dst = __uint_as_float(ld_shared_u32(staging + (uint32_t)(rr * kStorePitch + lane) * 4));
+            }
+        } else {
+            const int c = col + 2 * lane;
+            uint16_t* dst = static_cast<uint16_t*>(p.C) + (int64_t)row0 * p.ldc + c;
+#pragma unroll 8
+            for (int rr = 0; rr < rows; ++rr, dst += p.ldc) {
+                const uint32_t at = staging + (uint32_t)(rr * kStorePitch + lane) * 4;
+                const uint32_t v = ld_shared_u32(at);
+                if ((reinterpret_cast<uintptr_t>(dst) & 3u) == 0) {   // the same for the whole warp
+                    if (c + 1 < p.N) *reinterpret_cast<uint32_t*>(dst) = v;
+                    else if (c < p.N) dst[0] = (uint16_t)v;
                 } else {
-                    if (c < p.N) dst[0] = (uint16_t)v;
-                    if (c + 1 < p.N) dst[1] = (uint16_t)(v >> 16);
+                    if (lane == 0 && c < p.N) dst[0] = (uint16_t)v;
+                    if (lane < 31 && c + 2 < p.N) *reinterpret_cast<uint32_t*>(dst + 1) = __byte_perm(v, ld_shared_u32(at + 4), 0x5432);
+                    else if (c + 1 < p.N) dst[1] = (uint16_t)(v >> 16);
                 }
             }
         }
@@ -271,7 +316,7 @@ mx_matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
             constexpr int kStep = 128;
             for (int t = unit; t < num_tiles && !stopped && !*abort_flag; t += num_units) {
                 int tm, tn;
-                tile_coords(t, num_m, num_n, tm, tn);
+                mx_tile_coords(t, num_m, num_n, tm, tn);
                 const int row0 = (tm * G + (int)cta_rank) * 128;
                 const int col0 = tn * BN + (int)cta_rank * Cfg::kBNCta;
                 for (int kt = 0; kt < ktiles; ++kt) {
@@ -347,12 +392,12 @@ mx_matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
         const int quad = warp & 3;
         const int half = (warp - 2) >> 2;
         constexpr int CW = BN / 2;
-        const uint32_t staging = smem_store + (uint32_t)(warp - 2) * kStoreWarpBytes;
+        const uint32_t staging = Cfg::kAligned ? 0u : smem_store + (uint32_t)(warp - 2) * kStoreWarpBytes;
         const uint32_t acc_empty = (G == 2) ? mapa(bar_acc_empty, 0) : bar_acc_empty;
         int n = 0;
         for (int t = unit; t < num_tiles && !*abort_flag; t += num_units, ++n) {
             int tm, tn;
-            tile_coords(t, num_m, num_n, tm, tn);
+            mx_tile_coords(t, num_m, num_n, tm, tn);
             if (!__all_sync(0xFFFFFFFFu, mbar_wait(bar_acc_full, (uint32_t)n & 1u, p.wait_limit_ns))) {
                 if (lane == 0) report_timeout(p.status, abort_flag, 4);
                 break;
@@ -362,8 +407,8 @@ mx_matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
             const int row0 = (tm * G + (int)cta_rank) * 128 + 32 * quad;
             const int col = tn * BN + half * CW;
             // The 32 columns that both accumulators cover are the first's last ones and the second's first ones: the warp
-            // that owns them reads them first and hands them back; every warp arrives, whether it has a share or not.
-            const int first = (n & 1) ? 0 : CW - 32;
+            // that owns them reads its 64 columns with them first and hands them back; every warp arrives, whether it has a
+            // share or not.
             const bool shares = half == ((n & 1) ? 0 : 1);
             if (!shares) {
                 tc_fence_before();   // its reads of the tile before
@@ -371,17 +416,20 @@ mx_matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
                 if (lane == 0) mbar_arrive_cluster(acc_empty);
             }
 #pragma unroll 1
-            for (int i = 0; i < CW / 32; ++i) {
-                const int c = i == 0 ? first : (n & 1) ? 32 * i : 32 * (i - 1);
-                uint32_t r[32];
-                tc_ld_32x32b_x32(tacc + (uint32_t)c, r);
+            for (int i = 0; i < CW / 64; ++i) {
+                const int c = (n & 1) ? 64 * i : CW - 64 - 64 * i;
+                uint32_t r[64];
+                tc_ld_32x32b_x64(tacc + (uint32_t)c, r);
                 tc_wait_ld();
                 if (shares && i == 0) {
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive_cluster(acc_empty);
                 }
-                mx_store32(p, row0, col + c, r, staging, lane);
+                if (row0 < p.M && col + c < p.N) {   // the same for the whole warp
+                    if constexpr (Cfg::kAligned) mx_store_aligned(p, row0, col + c, r, lane);
+                    else mx_store_any(p, row0, col + c, r, staging, lane);
+                }
                 __syncwarp();
             }
         }
@@ -402,7 +450,7 @@ mx_matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
 //
 // With few rows on one side (a decoding step) the product is the reading of the other side's codes.  That side
 // ("long") takes the 128 rows of the MMA, the few rows its NT columns, and K is split over the S CTAs of a cluster so
-// that all SMs read: each CTA multiplies its share of the k-tiles, leaves its partial sums (fp32) in its shared
+// that all SMs read; a product of any size that has too few 128 x 128 tiles for the SMs is split the same way.  Each CTA multiplies its share of the k-tiles, leaves its partial sums (fp32) in its shared
 // memory, and each then adds 1 / S of the columns over the S CTAs, in the order of their ranks, and stores them.
 // No workspace, no atomics, one launch, the same sums whatever order the CTAs run in.
 
@@ -457,9 +505,9 @@ __device__ __forceinline__ void few_store(const FewParams& p, int i, int j, floa
 // This CTA's share of the columns (every S-th), four rows per thread and step: sums of the S partial sums.  The S loads
 // of a step do not wait for one another (one at a time cost 35 us of 75 with 128 rows and S = 2).
 template <int S>
-__device__ __forceinline__ void few_reduce(const FewParams& p, uint32_t sums, int rank, int row0, int thread)
+__device__ __forceinline__ void few_reduce(const FewParams& p, uint32_t sums, int rank, int row0, int j0, int columns, int thread)
 {
-    for (int it = thread; it < 32 * ((p.n_few - rank + S - 1) / S); it += 128) {
+    for (int it = thread; it < 32 * ((columns - rank + S - 1) / S); it += 128) {
         const int j = rank + S * (it >> 5), row = (it & 31) * 4;
         float4 v[S];
 #pragma unroll
@@ -471,10 +519,10 @@ __device__ __forceinline__ void few_reduce(const FewParams& p, uint32_t sums, in
             v[0].z += v[r].z;
             v[0].w += v[r].w;
         }
-        few_store(p, row0 + row, j, v[0].x);
-        few_store(p, row0 + row + 1, j, v[0].y);
-        few_store(p, row0 + row + 2, j, v[0].z);
-        few_store(p, row0 + row + 3, j, v[0].w);
+        few_store(p, row0 + row, j0 + j, v[0].x);
+        few_store(p, row0 + row + 1, j0 + j, v[0].y);
+        few_store(p, row0 + row + 2, j0 + j, v[0].z);
+        few_store(p, row0 + row + 3, j0 + j, v[0].w);
     }
 }
 
@@ -503,6 +551,7 @@ mx_matmul_few_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
     const int split = (int)gridDim.x;                 // the cluster spans the grid's x
     const int rank = (int)blockIdx.x;
     const int row0 = (int)blockIdx.y * 128;
+    const int j0 = (int)blockIdx.z * NT, columns = min(NT, p.n_few - j0);   // more than one z: NT = 128
     const int kt0 = (int)((int64_t)p.ktiles * rank / split), kt1 = (int)((int64_t)p.ktiles * (rank + 1) / split);
 
     if (threadIdx.x == 0) {
@@ -544,8 +593,8 @@ mx_matmul_few_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
                 mbar_arrive_expect_tx(full, p.tx_bytes);
                 tma_load_2d(smem_a + s * Cfg::kABytes, &tm_a, kt * 128, row0, full);
                 tma_load_3d<1>(smem_sa + s * Cfg::kSBytes, &tm_sa, 0, kt * Cfg::kChunks, row0 / 128, full);
-                tma_load_2d(smem_b + s * Cfg::kBBytes, &tm_b, kt * 128, 0, full);
-                tma_load_3d<1>(smem_sb + s * Cfg::kSBytes, &tm_sb, 0, kt * Cfg::kChunks, 0, full);
+                tma_load_2d(smem_b + s * Cfg::kBBytes, &tm_b, kt * 128, j0, full);
+                tma_load_3d<1>(smem_sb + s * Cfg::kSBytes, &tm_sb, 0, kt * Cfg::kChunks, j0 / 128, full);
                 if (++s == ST) { s = 0; ph ^= 1u; }
             }
         }
@@ -589,13 +638,13 @@ mx_matmul_few_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
             const uint32_t tacc = tmem_base + ((uint32_t)(32 * quad) << 16);
 #pragma unroll
             for (int c = 0; c < NT; c += 16) {
-                if (c >= p.n_few) break;
+                if (c >= columns) break;
                 uint32_t r[16];
                 tc_ld_32x32b_x16(tacc + (uint32_t)c, r);
                 tc_wait_ld();
                 if (split == 1) {
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) few_store(p, row0 + row, c + j, __uint_as_float(r[j]));
+                    for (int j = 0; j < 16; ++j) few_store(p, row0 + row, j0 + c + j, __uint_as_float(r[j]));
                 } else {   // every copy into the stages and every MMA that reads them is done
 #pragma unroll
                     for (int j = 0; j < 16; ++j) st_shared_u32(smem_base + (uint32_t)((c + j) * 128 + row) * 4, r[j]);
@@ -612,9 +661,9 @@ mx_matmul_few_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
         cluster_sync();
         if (warp >= 2) {
             const int thread = (int)threadIdx.x - 64;
-            if (split == 2) few_reduce<2>(p, smem_base, rank, row0, thread);
-            else if (split == 4) few_reduce<4>(p, smem_base, rank, row0, thread);
-            else few_reduce<8>(p, smem_base, rank, row0, thread);
+            if (split == 2) few_reduce<2>(p, smem_base, rank, row0, j0, columns, thread);
+            else if (split == 4) few_reduce<4>(p, smem_base, rank, row0, j0, columns, thread);
+            else few_reduce<8>(p, smem_base, rank, row0, j0, columns, thread);
         }
         __syncwarp();
         cluster_sync();   // nobody leaves while another reads its sums
@@ -682,7 +731,7 @@ static int launch_mx(const MxOperand& a, const MxOperand& b, MxParams p, cudaStr
         }
     }
     const int64_t tiles = (int64_t)((p.M + 128 * Cfg::kG - 1) / (128 * Cfg::kG)) * ((p.N + Cfg::kBN - 1) / Cfg::kBN);
-    if (tiles > 0x7FFFFFFFll / kGroupM) return fail(S24_ERR_SHAPE, "mx_matmul: too many output tiles");
+    if (tiles > 0x7FFFFFFFll / kMxGroupM) return fail(S24_ERR_SHAPE, "mx_matmul: too many output tiles");
     int units = sm_count() / Cfg::kG;
     if (units > tiles) units = (int)tiles;
     return check_cuda(mx::launch_overlapped(mx_matmul_kernel<Cfg>, dim3((unsigned)(units * Cfg::kG)), kMxThreads, Cfg::kSmemBytes, Cfg::kG, stream, tm_a, tm_b,
@@ -725,10 +774,9 @@ static int launch_few(const MxOperand& a, const MxOperand& b, FewParams p, int64
             if (dev >= 0 && dev < 64) opted_in[dev] = true;
         }
     }
-    const int tiles = (p.n_long + 127) / 128;
-    if (split == 0) split = few_split(tiles, p.ktiles);
+    const int tiles = (p.n_long + 127) / 128, across = (p.n_few + Cfg::kNT - 1) / Cfg::kNT;
     if (split > p.ktiles) split = 1;
-    return check_cuda(mx::launch_overlapped(mx_matmul_few_kernel<Cfg>, dim3((unsigned)split, (unsigned)tiles), kFewThreads, Cfg::kSmemBytes, (unsigned)split, stream,
+    return check_cuda(mx::launch_overlapped(mx_matmul_few_kernel<Cfg>, dim3((unsigned)split, (unsigned)tiles, (unsigned)across), kFewThreads, Cfg::kSmemBytes, (unsigned)split, stream,
                                             tm_a, tm_b, tm_sa, tm_sb, p),
                       "mx_matmul launch");
 }
@@ -736,7 +784,8 @@ static int launch_few(const MxOperand& a, const MxOperand& b, FewParams p, int64
 template <bool F4>
 static int run_few(const MxOperand& a, const MxOperand& b, const MxParams& p, int split, cudaStream_t stream)
 {
-    const bool swap = p.M <= p.N;   // the few rows are A's
+    // the few rows are A's, and A's too where neither side's are few: then a warp's 32 rows of B are neighbours in C
+    const bool swap = p.M <= p.N || p.N > 128;
     const MxOperand& lng = swap ? b : a;
     const MxOperand& few = swap ? a : b;
     FewParams f;
@@ -762,41 +811,73 @@ static int run_few(const MxOperand& a, const MxOperand& b, const MxParams& p, in
 // and pass over the SMs, in microseconds as measured with the operands in L2 at 256 rows and K of 512 to 16384.  What the
 // memory bounds, it bounds for all of them alike.  Measured against it (tiles 256 x 256, 256 x 128, 128 x 128):
 // 256 x 8192 x 8192 4-bit 17.4 / 13.6 / 14.7 us, 512 x 8192 x 8192 8-by-4-bit 28.0 / 30.5 / 34.6, 160 x 1000 x 1024 8-bit
-// 20.5 / 13.7 / 13.1; few rows, against the best tile: 64 x 28672 x 8192 30.7 / 35.7, 128 x 28672 x 8192 39.1 / 36.7,
-// 128 x 4096 x 16384 18.4 / 26.6.
+// 20.5 / 13.7 / 13.1.  K split over a cluster against the best tile: 64 x 28672 x 8192 30.7 / 35.7, 128 x 28672 x 8192
+// 39.1 / 36.7, 129 x 1000 x 16384 12.6 / 27.0, 300 x 1300 x 8192 12.3 / 17.4, 512 x 512 x 4096 7.9 / 6.2.
+struct MxPlan {
+    double time;
+    int bm, bn, split;   // split > 0: the kernel for few rows
+};
+
+static MxPlan plan_few(int64_t few, int64_t lng, int ktiles)
+{
+    const int n = (int)((lng + 127) / 128 * ((few + 127) / 128)), s = few_split(n, ktiles);
+    const double passes = (double)((n * s + 2 * sm_count() - 1) / (2 * sm_count()));
+    const double per_ktile = (few > 64 ? 0.36 : 0.25) * (n * s > sm_count() ? 2.0 : 1.0);
+    return {(few > 64 ? 7.6 : 3.0) + passes * ktiles / s * per_ktile, 0, 0, s};
+}
+
+static MxPlan plan_mx(int64_t M, int64_t N, int ktiles)
+{
+    const int64_t few = M < N ? M : N, lng = M < N ? N : M;
+    // the long side's tiles are the grid's y; K is split where there are fewer tiles than SMs, or few rows
+    const bool few_ok = few <= 128 ? lng <= 65535 * 128 : ((M + 127) / 128) * ((N + 127) / 128) <= sm_count();
+    if (few_ok && few <= 64) return plan_few(few, lng, ktiles);
+    struct Tile { int bm, bn, units; double fixed, per_ktile, per_pass; };
+    const Tile tiles[3] = {{256, 256, sm_count() / 2, 5.7, 0.29, 0.0}, {256, 128, sm_count() / 2, 4.7, 0.185, 0.6}, {128, 128, sm_count(), 4.3, 0.21, 0.6}};
+    MxPlan best = {1e30, 0, 0, 0};
+    for (const Tile& t : tiles) {
+        const int64_t n = ((M + t.bm - 1) / t.bm) * ((N + t.bn - 1) / t.bn);
+        const double passes = (double)((n + t.units - 1) / t.units);
+        const double time = t.fixed + passes * ktiles * t.per_ktile + (passes - 1) * t.per_pass;
+        if (time < best.time) best = {time, t.bm, t.bn, 0};
+    }
+    if (few_ok) {
+        const MxPlan f = plan_few(few, lng, ktiles);
+        if (f.time < best.time) best = f;
+    }
+    return best;
+}
+
+template <bool F4>
+static int launch_plan(const MxOperand& a, const MxOperand& b, const MxParams& p, const MxPlan& plan, cudaStream_t stream)
+{
+    if (plan.split > 0) return run_few<F4>(a, b, p, plan.split, stream);
+    if (p.wide) {
+        if (plan.bm == 256 && plan.bn == 256) return launch_mx<MxCfg<2, 256, F4, 6, true>>(a, b, p, stream);
+        if (plan.bm == 256 && plan.bn == 128) return launch_mx<MxCfg<2, 128, F4, 8, true>>(a, b, p, stream);
+        if (plan.bm == 128 && plan.bn == 128) return launch_mx<MxCfg<1, 128, F4, 6, true>>(a, b, p, stream);
+    } else {
+        if (plan.bm == 256 && plan.bn == 256) return launch_mx<MxCfg<2, 256, F4, 5, false>>(a, b, p, stream);
+        if (plan.bm == 256 && plan.bn == 128) return launch_mx<MxCfg<2, 128, F4, 7, false>>(a, b, p, stream);
+        if (plan.bm == 128 && plan.bn == 128) return launch_mx<MxCfg<1, 128, F4, 5, false>>(a, b, p, stream);
+    }
+    return fail(S24_ERR_UNSUPPORTED, "mx_matmul: no kernel for tile %d x %d (have 256x256, 256x128, 128x128)", plan.bm, plan.bn);
+}
+
 template <bool F4>
 static int pick_mx(const MxOperand& a, const MxOperand& b, const MxParams& p, const s24_tile_cfg* cfg, cudaStream_t stream)
 {
-    int bm = cfg ? cfg->bm : 0, bn = cfg ? cfg->bn : 0;
-    const int few = p.M < p.N ? p.M : p.N, lng = p.M < p.N ? p.N : p.M;
-    const bool few_ok = few <= 128 && lng <= 65535 * 128;   // the long side's tiles are the grid's y
-    const int split = cfg ? cfg->split : 0;
-    if (split != 0 && (!few_ok || (split != 1 && split != 2 && split != 4 && split != 8)))
-        return fail(S24_ERR_UNSUPPORTED, "mx_matmul: K can be split 1, 2, 4 or 8 ways, with at most 128 rows on one side (got %d)", split);
-    if (split != 0) return run_few<F4>(a, b, p, split, stream);
-    if (bm == 0 && bn == 0) {
-        if (few_ok && few <= 64) return run_few<F4>(a, b, p, 0, stream);
-        struct Tile { int bm, bn, units; double fixed, per_ktile, per_pass; };
-        const Tile tiles[3] = {{256, 256, sm_count() / 2, 5.7, 0.29, 0.0}, {256, 128, sm_count() / 2, 4.7, 0.185, 0.6}, {128, 128, sm_count(), 4.3, 0.21, 0.6}};
-        const double ktiles = (double)((p.K + (F4 ? 255 : 127)) / (F4 ? 256 : 128));
-        double least = 1e30;
-        for (const Tile& t : tiles) {
-            const int64_t n = (((int64_t)p.M + t.bm - 1) / t.bm) * (((int64_t)p.N + t.bn - 1) / t.bn);
-            const double passes = (double)((n + t.units - 1) / t.units);
-            const double time = t.fixed + passes * ktiles * t.per_ktile + (passes - 1) * t.per_pass;
-            if (time < least) { least = time; bm = t.bm; bn = t.bn; }
-        }
-        if (few_ok) {
-            const int n = (lng + 127) / 128, s = few_split(n, (int)ktiles);
-            if (n * s <= 2 * sm_count() && 6.5 + ktiles / s * (n * s > sm_count() ? 0.72 : 0.36) < least) return run_few<F4>(a, b, p, s, stream);
-        }
+    const int ktiles = (p.K + (F4 ? 255 : 127)) / (F4 ? 256 : 128);
+    if (cfg != nullptr && (cfg->bm != 0 || cfg->bn != 0 || cfg->split != 0)) {
+        const int few = p.M < p.N ? p.M : p.N, lng = p.M < p.N ? p.N : p.M, split = cfg->split;
+        if (split != 0 && (few > 8192 || lng > 65535 * 128 || (split != 1 && split != 2 && split != 4 && split != 8)))
+            return fail(S24_ERR_UNSUPPORTED, "mx_matmul: K can be split 1, 2, 4 or 8 ways, with at most 8192 rows on one side (got %d)", split);
+        MxPlan plan = {0.0, cfg->bm, cfg->bn, split};
+        if (plan.bm == 0) plan.bm = plan.bn == 256 || p.M > 128 ? 256 : 128;
+        if (plan.bn == 0) plan.bn = 128;
+        return launch_plan<F4>(a, b, p, plan, stream);
     }
-    if (bm == 0) bm = bn == 256 || p.M > 128 ? 256 : 128;
-    if (bn == 0) bn = 128;
-    if (bm == 256 && bn == 256) return launch_mx<MxCfg<2, 256, F4, 6>>(a, b, p, stream);
-    if (bm == 256 && bn == 128) return launch_mx<MxCfg<2, 128, F4, 8>>(a, b, p, stream);
-    if (bm == 128 && bn == 128) return launch_mx<MxCfg<1, 128, F4, 6>>(a, b, p, stream);
-    return fail(S24_ERR_UNSUPPORTED, "mx_matmul: no kernel for tile %d x %d (have 256x256, 256x128, 128x128)", bm, bn);
+    return launch_plan<F4>(a, b, p, plan_mx(p.M, p.N, ktiles), stream);
 }
 
 }  // namespace s24

@@ -135,8 +135,8 @@ typedef struct s24_tile_cfg {
     int bn;        /* columns per tile: 128 or 256; 224 with bm = 512; 0 = auto */
     int stages;    /* reserved, ignored: every tile shape has one ring depth (512x224: 3, 256x256: 4,
                       256x128: 6, 128x128: 4 stages of K = 128) that fills the 227 KB of shared memory */
-    int split;     /* s24_mx_matmul only, others ignore it: with at most 128 rows on one side, the number of CTAs that
-                      share K (1, 2, 4 or 8); 0 = auto */
+    int split;     /* s24_mx_matmul only, others ignore it: number of CTAs that share K (1, 2, 4 or 8), on tiles of 128 x 128
+                      or less, with at most 8192 rows on one side; 0 = auto */
 } s24_tile_cfg;
 
 S24_API int s24_version(void);
@@ -343,7 +343,7 @@ S24_API int s24_mx_rms_norm(const void* x, const void* residual, const void* wei
  * S24_SCALES_TC order.  K % 32 == 0, and K % 128 == 0 where the formats differ; any M and N.  Codes:
  * rows and pointers on 16 bytes, a S24_MXFP4 operand beside a S24_MXFP8 one on 32; scales on 16; C on its
  * element.  Two operands of 4 bits run at twice the rate of the other pairs.  cfg: tiles 256 x 256 and
- * 256 x 128 (CTA pair) or 128 x 128, or a split of K for few rows.
+ * 256 x 128 (CTA pair) or 128 x 128, or a split of K.
  */
 S24_API int s24_mx_matmul(const void* a, const void* a_scales, const void* b, const void* b_scales, void* C,
                   int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb, int64_t ldc,

@@ -192,21 +192,22 @@ def _operand(s24, r, k, fmt, seed, exact):
 
 
 PAIRS = [("mxfp4", "mxfp4"), ("mxfp8", "mxfp8"), ("mxfp8", "mxfp4"), ("mxfp4", "mxfp8")]
-SPLITS = [{"SPLIT": 1}, {"SPLIT": 2}, {"SPLIT": 4}, {"SPLIT": 8}]    # the kernel for few rows, K split over that many CTAs
+SPLITS = [{"SPLIT": 1}, {"SPLIT": 2}, {"SPLIT": 4}, {"SPLIT": 8}]    # K split over that many CTAs
 TILES = [None, {"BM": 128, "BN": 128}, {"BM": 256, "BN": 128}, {"BM": 256, "BN": 256}]
 
 
 @pytest.mark.parametrize("fa,fb", PAIRS)
 @pytest.mark.parametrize("m,n,k", [(1, 1, 32), (1, 8, 128), (3, 5, 96), (1, 257, 256), (2, 1000, 1024), (17, 130, 384), (40, 520, 2048), (64, 64, 160),
                                    (100, 4099, 512), (128, 128, 128), (129, 127, 256), (200, 333, 640), (256, 256, 512), (257, 515, 416), (1000, 300, 1024),
-                                   (2048, 1544, 512), (513, 2049, 128)])
+                                   (2048, 1544, 512), (513, 2049, 128),
+                                   (1537, 6150, 1024), (1540, 6144, 512), (6200, 1536, 512)])
 def test_product_is_exact_where_sums_are(s24, m, n, k, fa, fb):
     if fa != fb:
         k = -(-k // 128) * 128
     a, sa, va = _operand(s24, m, k, fa, 1000 * m + k, True)
     b, sb, vb = _operand(s24, n, k, fb, 1000 * n + k + 1, True)
     want = torch.from_numpy(va) @ torch.from_numpy(vb).t()      # below 2^6 * 2048 * ..., whole multiples of 2^-6: exact in fp32
-    for tile in TILES + (SPLITS if min(m, n) <= 128 else []):
+    for tile in TILES + SPLITS:
         got = s24.mx_matmul(a, sa, b, sb, out_dtype=torch.float32, manual_config=tile)
         assert torch.equal(got.cpu().double(), want), f"tile {tile}: {(got.cpu().double() != want).sum()} of {want.numel()} differ"
     for out in (torch.bfloat16, torch.float16):
@@ -315,4 +316,35 @@ def test_a_chain_of_them_on_another_stream_and_in_a_graph(s24):
             graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(out, eager) for _, out in graphs)
+    assert s24.lib().s24_device_status(None) == 0
+
+
+def test_offsets_beyond_32_bits(s24):
+    """operands, scales and results whose last rows lie past 4 GB: the same bits as for those rows by themselves"""
+    r, k = 140032, 16384                                   # 4.6 GB in 16 bits
+    x = torch.empty(r, k, dtype=torch.bfloat16, device=DEV)
+    tail = torch.randn(128, k, generator=torch.Generator(device=DEV).manual_seed(2), device=DEV).to(torch.bfloat16)
+    x.zero_()
+    x[-128:] = tail
+    codes, scales, tc = s24.mx_quantize(x, "mxfp8", want_tc=True)
+    c2, s2, t2 = s24.mx_quantize(tail, "mxfp8", want_tc=True)
+    assert torch.equal(codes[-128:].view(torch.uint8), c2.view(torch.uint8)) and torch.equal(scales[-128:], s2) and torch.equal(tc[-t2.numel():], t2)
+    w = torch.ones(k, dtype=torch.bfloat16, device=DEV)
+    n1, n2 = s24.mx_rms_norm(x, w, residual=x), s24.mx_rms_norm(tail, w, residual=tail)
+    for a, b in zip(n1, n2):
+        assert (a is None) == (b is None) and (a is None or torch.equal(a[-128:].view(torch.uint8), b.view(torch.uint8)))
+    del n1, x
+    back = s24.mx_dequantize(codes, scales, dtype=torch.bfloat16)
+    assert torch.equal(back[-128:], s24.mx_dequantize(c2, s2, dtype=torch.bfloat16))
+    del back
+    b, _, bt = s24.mx_quantize(tail[:, :].contiguous(), "mxfp8", False, True)
+    few = s24.mx_matmul(b[:3], s24.mx_quantize(tail[:3], "mxfp8", False, True)[2], codes, tc)        # (3, r): rows of the long side past 2 GB
+    assert torch.equal(few[:, -128:], s24.mx_matmul(b[:3], s24.mx_quantize(tail[:3], "mxfp8", False, True)[2], c2, t2))
+    del codes, scales, tc
+    # a result past 4 GB, through the tiles: its last block against the product of those rows
+    a8, _, a8t = s24.mx_quantize(torch.randn(70016, 128, device=DEV).to(torch.bfloat16), "mxfp4", False, True)
+    b8, _, b8t = s24.mx_quantize(torch.randn(32896, 128, device=DEV).to(torch.bfloat16), "mxfp4", False, True)
+    c = s24.mx_matmul(a8, a8t, b8, b8t)
+    one = s24.mx_matmul(a8[-128:], a8t[-512:], b8[-128:], b8t[-512:])
+    assert torch.equal(c[-128:, -128:], one)
     assert s24.lib().s24_device_status(None) == 0
