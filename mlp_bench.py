@@ -8,6 +8,9 @@ by an NCCL all-gather, and with one made by the GEMM storing each shard into all
 
 Rank 0 prints one JSON line: aggregate dense-equivalent TFLOP/s (max-over-ranks device time)
 for the sharded result and for the two replicated ones.
+
+--mx compresses by number format instead: W in 4-bit microscaled form, X^T (the tokens of this rank's
+shard, 8192 wide) quantised to 8 bits inside the timed step, then their product, sharded the same way.
 """
 from __future__ import annotations
 
@@ -32,6 +35,7 @@ def main():
     ap = argparse.ArgumentParser()
     ap.add_argument("--steps", type=int, default=10)
     ap.add_argument("--gather-steps", type=int, default=3)
+    ap.add_argument("--mx", action="store_true", help="microscaled formats instead of 2:4 sparsity")
     args = ap.parse_args()
     rank, world, local = int(os.environ.get("RANK", 0)), int(os.environ.get("WORLD_SIZE", 1)), int(os.environ.get("LOCAL_RANK", 0))
     torch.cuda.set_device(local)
@@ -41,11 +45,14 @@ def main():
     g = torch.Generator(device=dev).manual_seed(5000)                    # same W on every rank
     W = (0.02 * torch.randn(M, K, generator=g, device=dev, dtype=torch.float32)).to(torch.bfloat16)
     vals, _, tc = s24.prune_compress(W, want_ref=False, want_tc=True)    # compressed redundantly, no broadcast
+    W4, _, W4_tc = s24.mx_quantize(W, "mxfp4", want_rows=False, want_tc=True) if args.mx else (None, None, None)
     del W
     op = NShardedSpmm(vals, tc)
     n0, n1 = op.local_columns(N)
     gx = torch.Generator(device=dev).manual_seed(5001 + rank)
     X = torch.randn(K, n1 - n0, generator=gx, device=dev, dtype=torch.float32).to(torch.bfloat16)
+    if args.mx:
+        X = X.t().contiguous()
     stream = torch.cuda.current_stream(dev)
 
     def barrier():
@@ -70,6 +77,19 @@ def main():
         return float(t.item())
 
     flops = 2.0 * M * N * K
+    if args.mx:
+        def mx_step():
+            codes, _, scales = s24.mx_quantize(X, "mxfp8", want_rows=False, want_tc=True)
+            return s24.mx_matmul(codes, scales, W4, W4_tc)
+
+        ms = timed(mx_step, args.steps)
+        op.close()
+        if rank == 0:
+            print(json.dumps({"workload": f"X {N}x{K} bf16 -> mxfp8 . (W {M}x{K} mxfp4)^T, tokens sharded x{world}", "n_gpus": world,
+                              "mx": {"ms": ms, "tflops": flops / ms / 1e9}}), flush=True)
+        if world > 1:
+            dist.destroy_process_group()
+        return
     ms_shard = timed(lambda: op(X), args.steps)
     line = {"workload": f"W24 {M}x{K} bf16 . X {K}x{N} bf16, columns sharded x{world}", "n_gpus": world,
             "sharded": {"ms": ms_shard, "tflops": flops / ms_shard / 1e9}}
