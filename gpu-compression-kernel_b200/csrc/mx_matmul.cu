@@ -198,13 +198,15 @@ __device__ __forceinline__ void mx_store_aligned(const MxParams& p, int row0, in
     }
 }
 
-// The same for rows that start anywhere: through shared memory, so that 32 lanes write 128 bytes of one row.  16-bit rows
-// that start on an odd element are written as words from their second element on.  (32 bytes of four rows at a time took
-// 52.9 us at 1537 x 6150 x 4128, this 50.8; without any stores it is 42.2.)
+// The same for rows that start anywhere: through shared memory, so that 32 lanes write 128 bytes of one row.  Of 16-bit
+// rows every second starts on the same half of a word: rows that start on a whole word are written as words, the others
+// as words from their second element on, with their first and last elements by themselves.
 __device__ __forceinline__ void mx_store_any(const MxParams& p, int row0, int col, const uint32_t (&r)[64], uint32_t staging, int lane)
 {
     const bool f32 = p.out == S24_FP32;
     const int rows = min(32, p.M - row0);   // the same for the whole warp
+    const uint32_t own = staging + (uint32_t)lane * 4;
+    constexpr uint32_t kRow = kStorePitch * 4;
 #pragma unroll
     for (int part = 0; part < 2; ++part) {
         if (part == 1 && !f32) break;
@@ -212,31 +214,48 @@ __device__ __forceinline__ void mx_store_any(const MxParams& p, int row0, int co
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
             const uint32_t w = f32 ? r[32 * part + i] : pack2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]), p.out == S24_BF16);
-            st_shared_u32(staging + (uint32_t)(lane * kStorePitch + i) * 4, w);
+            st_shared_u32(staging + (uint32_t)lane * kRow + 4 * i, w);
         }
         __syncwarp();
         if (f32) {
             const int c = col + 32 * part + lane;
             float* dst = static_cast<float*>(p.C) + (int64_t)row0 * p.ldc + c;
-            if (c < p.N) {
-#pragma unroll 8
-                for (int rr = 0; rr < rows; ++rr, dst += p.ldc) *dst = __uint_as_float(ld_shared_u32(staging + (uint32_t)(rr * kStorePitch + lane) * 4));
+            if (rows == 32 && col + 32 * part + 32 <= p.N) {
+#pragma unroll
+                for (int rr = 0; rr < 32; ++rr) dst[rr * p.ldc] = __uint_as_float(ld_shared_u32(own + rr * kRow));
+            } else if (c < p.N) {
+                for (int rr = 0; rr < rows; ++rr) dst[rr * p.ldc] = __uint_as_float(ld_shared_u32(own + rr * kRow));
+            }
+        } else if (rows == 32 && col + 64 <= p.N) {
+            uint16_t* first = static_cast<uint16_t*>(p.C) + (int64_t)row0 * p.ldc + col;
+#pragma unroll
+            for (int odd = 0; odd < 2; ++odd) {
+                uint16_t* start = first + odd * p.ldc;
+                const uint32_t from = own + odd * kRow;
+                if ((reinterpret_cast<uintptr_t>(start) & 3u) == 0) {   // the same for the whole warp
+                    uint32_t* dst = reinterpret_cast<uint32_t*>(start) + lane;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) dst[i * p.ldc] = ld_shared_u32(from + 2 * i * kRow);
+                } else {
+                    uint32_t* dst = reinterpret_cast<uint32_t*>(start + 1) + lane;
+                    if (lane < 31) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            dst[i * p.ldc] = __byte_perm(ld_shared_u32(from + 2 * i * kRow), ld_shared_u32(from + 2 * i * kRow + 4), 0x5432);
+                    }
+                    // lanes 0-15: the first elements of the 16 rows, 16-31: their last
+                    const int i = lane & 15, last = lane >> 4;
+                    const uint32_t w = ld_shared_u32(staging + (uint32_t)(odd + 2 * i) * kRow + (last ? 124u : 0u));
+                    start[(int64_t)(2 * i) * p.ldc + (last ? 63 : 0)] = (uint16_t)(last ? w >> 16 : w);
+                }
             }
         } else {
             const int c = col + 2 * lane;
             uint16_t* dst = static_cast<uint16_t*>(p.C) + (int64_t)row0 * p.ldc + c;
-#pragma unroll 8
             for (int rr = 0; rr < rows; ++rr, dst += p.ldc) {
-                const uint32_t at = staging + (uint32_t)(rr * kStorePitch + lane) * 4;
-                const uint32_t v = ld_shared_u32(at);
-                if ((reinterpret_cast<uintptr_t>(dst) & 3u) == 0) {   // the same for the whole warp
-                    if (c + 1 < p.N) *reinterpret_cast<uint32_t*>(dst) = v;
-                    else if (c < p.N) dst[0] = (uint16_t)v;
-                } else {
-                    if (lane == 0 && c < p.N) dst[0] = (uint16_t)v;
-                    if (lane < 31 && c + 2 < p.N) *reinterpret_cast<uint32_t*>(dst + 1) = __byte_perm(v, ld_shared_u32(at + 4), 0x5432);
-                    else if (c + 1 < p.N) dst[1] = (uint16_t)(v >> 16);
-                }
+                const uint32_t v = ld_shared_u32(own + rr * kRow);
+                if (c < p.N) dst[0] = (uint16_t)v;
+                if (c + 1 < p.N) dst[1] = (uint16_t)(v >> 16);
             }
         }
     }
