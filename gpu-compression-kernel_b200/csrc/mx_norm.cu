@@ -182,11 +182,11 @@ mx_rms_norm_kernel(const NormParams p)
         amax = max(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 1));
         const uint8_t* h_at = (p.residual != nullptr ? p.h + (int64_t)r * (p.KB * 64) : p.x + (int64_t)r * p.x_row_bytes) + at * 32;
         const uint8_t* w_at = p.weight + at * 32;
-        // a power of two too near to tell the scale, or numbers too small for fp32's own rounding
-        const bool unsure = ((amax + 8u) & 0x7FFFFFu) < 16u || amax - 1u < 0x0E800000u;
+        // a power of two too near to tell the scale, or numbers too small for fp32's own rounding; not a block of zeros
+        const bool unsure = amax != 0u && (((amax + 8u) & 0x7FFFFFu) < 16u || amax <= 0x0E800000u);
         if (__any_sync(0xFFFFFFFFu, unsure)) {
             uint32_t exact = 0;
-            if (ok) {
+            if (ok && unsure) {
 #pragma unroll 1
                 for (int e = 0; e < 16; ++e) exact = max(exact, magnitude_bits(norm_exact<DT>(h_at + 2 * e, w_at + 2 * e, rhi, rlo)));
             }
