@@ -65,7 +65,9 @@ __device__ __forceinline__ float norm_exact(const uint8_t* h, const uint8_t* w, 
     const float t = hv * rhi;
     const float t_err = fmaf(hv, rlo, fmaf(hv, rhi, -t));
     const float v = t * wv;
-    return round_to_odd(v, fmaf(t_err, wv, fmaf(t, wv, -v)));
+    const float v_err = fmaf(t_err, wv, fmaf(t, wv, -v));   // as much as two units in the last place of v,
+    const float y = v + v_err;                              // so the pair is brought to a nearest value and its rest
+    return round_to_odd(y, v_err - (y - v));
 }
 
 // codes of a piece times up

@@ -348,3 +348,26 @@ def test_offsets_beyond_32_bits(s24):
     one = s24.mx_matmul(a8[-128:], a8t[-512:], b8[-128:], b8t[-512:])
     assert torch.equal(c[-128:, -128:], one)
     assert s24.lib().s24_device_status(None) == 0
+
+
+@pytest.mark.parametrize("fmt", ["mxfp8", "mxfp4"])
+@pytest.mark.parametrize("seed", [1, 2])
+def test_norm_of_many_elements_is_the_formula_in_64_bits(s24, seed, fmt):
+    """134 million elements, of which several lie within a unit in the last place of a border: every code and scale"""
+    r, k = 16384, 8192
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    x = torch.randn(r, k, generator=g, device=DEV).mul_(torch.exp(0.5 * torch.randn(k, generator=g, device=DEV))).to(torch.bfloat16)
+    w = (1 + 0.1 * torch.randn(k, generator=g, device=DEV)).to(torch.bfloat16)
+    codes, scales, _, _ = s24.mx_rms_norm(x, w, eps=1e-6, residual=x, fmt=fmt)
+    emax, top = (2, 6.0) if fmt == "mxfp4" else (8, 448.0)
+    low, fraction = (0, 1) if fmt == "mxfp4" else (-6, 3)
+    for i in range(0, r, 2048):
+        h = (2 * x[i:i + 2048].float()).to(torch.bfloat16).double()
+        y = (h / torch.sqrt((h * h).sum(-1, keepdim=True) / k + 1e-6) * w.double()).view(2048, k // 32, 32)
+        s = torch.frexp(y.abs().amax(-1))[1] - 1 - emax
+        assert torch.equal(scales[i:i + 2048].int() - 127, s.int())
+        u = torch.ldexp(y, -s.unsqueeze(-1))
+        step = torch.ldexp(torch.ones_like(u), (torch.frexp(u.abs())[1] - 1).clamp(min=low) - fraction)
+        q = (torch.round(u / step) * step).clamp(-top, top)
+        got = s24.mx_dequantize(codes[i:i + 2048], torch.full_like(scales[i:i + 2048], 127), dtype=torch.float32).view_as(q)
+        assert int((got.double() != q).sum()) == 0
