@@ -20,7 +20,7 @@ namespace s24 {
 
 using namespace mx;
 
-// value + error, |error| below one unit in the last place of value, rounded to odd
+// value + error, where value is the nearest fp32 number to the sum, rounded to odd
 __device__ __forceinline__ float round_to_odd(float value, float error)
 {
     const uint32_t b = __float_as_uint(value), e = __float_as_uint(error);

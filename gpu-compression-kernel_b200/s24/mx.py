@@ -31,7 +31,9 @@ _EMPTY = {}   # (device index, type) -> a tensor without elements
 def _new(device: int, dtype: torch.dtype, *shape: int) -> torch.Tensor:
     e = _EMPTY.get((device, dtype))
     if e is None:
-        e = _EMPTY[(device, dtype)] = torch.empty(0, dtype=dtype, device=torch.device("cuda", device))
+        e = torch.empty(0, dtype=dtype, device=torch.device("cuda", device))
+        if type(e) is torch.Tensor:   # not one that a dispatch mode put in its place
+            _EMPTY[(device, dtype)] = e
     return e.new_empty(*shape)
 
 

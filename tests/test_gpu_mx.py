@@ -97,6 +97,29 @@ def test_quantize_takes_strided_unaligned_and_higher_dimensional_inputs(s24):
         assert np.array_equal(tc.cpu().numpy(), mxo.tc_order(want_s))
 
 
+def test_refusals_on_the_gpu(s24):
+    x = torch.zeros(8, 64, dtype=torch.bfloat16, device=DEV)
+    w = torch.ones(64, dtype=torch.bfloat16, device=DEV)
+    with pytest.raises(RuntimeError, match="at least one layout"):
+        s24.mx_quantize(x, want_rows=False)
+    with pytest.raises(RuntimeError, match="at least one layout"):
+        s24.mx_rms_norm(x, w, want_rows=False)
+    for eps in (0.0, -1.0, float("nan"), float("inf")):
+        with pytest.raises(s24.S24Error, match="eps must be"):
+            s24.mx_rms_norm(x, w, eps=eps)
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        s24.mx_rms_norm(x, w.cpu())
+    codes, scales, tc = s24.mx_quantize(x, want_tc=True)
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        s24.mx_dequantize(codes, scales.cpu())
+    with pytest.raises(RuntimeError, match="contiguous bytes"):
+        s24.mx_matmul(codes, tc[:256], codes, tc)
+    for config in ({"BM": 64, "BN": 64}, {"BM": 128, "BN": 256}, {"SPLIT": 3}):
+        with pytest.raises(s24.S24Error):
+            s24.mx_matmul(codes, tc, codes, tc, manual_config=config)
+    torch.cuda.synchronize()
+
+
 def test_empty_inputs(s24):
     x = torch.empty(0, 64, dtype=torch.float16, device=DEV)
     codes, scales, tc = s24.mx_quantize(x, want_tc=True)
