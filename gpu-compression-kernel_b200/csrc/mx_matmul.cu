@@ -432,7 +432,7 @@ mx_matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
             if (!shares) {
                 tc_fence_before();   // its reads of the tile before
                 __syncwarp();
-                if (lane == 0) mbar_arrive_cluster(acc_empty);
+                if (lane == 0) mbar_arrive_remote(acc_empty);
             }
 #pragma unroll 1
             for (int i = 0; i < CW / 64; ++i) {
@@ -443,7 +443,7 @@ mx_matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
                 if (shares && i == 0) {
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive_cluster(acc_empty);
+                    if (lane == 0) mbar_arrive_remote(acc_empty);
                 }
                 if (row0 < p.M && col + c < p.N) {   // the same for the whole warp
                     if constexpr (Cfg::kAligned) mx_store_aligned(p, row0, col + c, r, lane);
