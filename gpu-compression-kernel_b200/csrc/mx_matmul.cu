@@ -364,13 +364,6 @@ mx_matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
             uint32_t ph = 0;
             bool ok = true;
             for (int t = unit; t < num_tiles && ok && !*abort_flag; t += num_units, ++n) {
-                // the epilogue has read what the previous tile's accumulator shares with this one's (and, before it, all
-                // of the tile before that, which had this accumulator)
-                if (n > 0 && !mbar_wait(bar_acc_empty, (uint32_t)(n - 1) & 1u, p.wait_limit_ns)) {
-                    report_timeout(p.status, abort_flag, 3);
-                    break;
-                }
-                tc_fence_after();
                 const uint32_t tmem_d = tmem_base + (uint32_t)((n & 1) * Cfg::kAccStep);
                 for (int kt = 0; kt < ktiles; ++kt) {
                     if (!mbar_wait(bar_full + 8 * s, ph, p.wait_limit_ns)) {
@@ -387,6 +380,16 @@ mx_matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
                         for (int b = 0; b < Cfg::kTilesB; ++b)
                             tc_cp_scales<G>(sfb + 4 * (c * Cfg::kTilesB + b),
                                             make_smem_desc(smem_sb + s * Cfg::kSBBytes + (b * Cfg::kChunks + c) * mx::kRecordBytes, 128, 128, kSwizzleNone));
+                    }
+                    // the epilogue has read what the previous tile's accumulator shares with this one's (and, before it, all
+                    // of the tile before that, which had this accumulator)
+                    if (kt == 0 && n > 0) {
+                        if (!mbar_wait(bar_acc_empty, (uint32_t)(n - 1) & 1u, p.wait_limit_ns)) {
+                            report_timeout(p.status, abort_flag, 3);
+                            ok = false;
+                            break;
+                        }
+                        tc_fence_after();
                     }
                     const uint64_t adesc = make_smem_desc(smem_a + s * Cfg::kABytes, 16, 1024, kSwizzle128B);
                     const uint64_t bdesc = make_smem_desc(smem_b + s * Cfg::kBBytes, 16, 1024, kSwizzle128B);
