@@ -394,3 +394,83 @@ def test_norm_of_many_elements_is_the_formula_in_64_bits(s24, seed, fmt):
         q = (torch.round(u / step) * step).clamp(-top, top)
         got = s24.mx_dequantize(codes[i:i + 2048], torch.full_like(scales[i:i + 2048], 127), dtype=torch.float32).view_as(q)
         assert int((got.double() != q).sum()) == 0
+
+
+def test_products_of_random_shapes(s24):
+    """shapes drawn over the whole range of tiles, splits and unaligned rows, windows of larger results among them"""
+    rng = np.random.default_rng(42)
+    for i in range(60):
+        fa, fb = PAIRS[int(rng.integers(4))]
+        m, n = (int(np.exp(rng.uniform(0, np.log(1500)))) for _ in range(2))
+        k = 128 * int(rng.integers(1, 13)) if fa != fb else 32 * int(rng.integers(1, 49))
+        out = DTYPES[int(rng.integers(3))]
+        a, sa, va = _operand(s24, m, k, fa, 10 * i, True)
+        b, sb, vb = _operand(s24, n, k, fb, 10 * i + 1, True)
+        want = (torch.from_numpy(va) @ torch.from_numpy(vb).t()).to(out)
+        pad, first = int(rng.integers(0, 40)), int(rng.integers(0, 8))
+        big = torch.full((m + 2, first + n + pad), 5.0, dtype=out, device=DEV)
+        s24.mx_matmul(a, sa, b, sb, out_dtype=out, out=big[1:m + 1, first:first + n])
+        full = torch.full((m + 2, first + n + pad), 5.0, dtype=out)
+        full[1:m + 1, first:first + n] = want
+        assert torch.equal(big.cpu(), full), (i, fa, fb, m, n, k, out, pad, first)
+        assert torch.equal(s24.mx_matmul(a, sa, b, sb, out_dtype=out).cpu(), want), (i, fa, fb, m, n, k, out)
+
+
+def test_two_streams_at_once(s24):
+    """products of every kind, norms and quantisations on two streams that run together: the bits of one stream alone"""
+    def work(seed):
+        g = torch.Generator(device=DEV).manual_seed(seed)
+        x = torch.randn(300, 2048, generator=g, device=DEV).to(torch.bfloat16)
+        w = torch.randn(1500, 2048, generator=g, device=DEV).to(torch.bfloat16)
+        gamma = torch.ones(2048, dtype=torch.bfloat16, device=DEV)
+        return x, w, gamma
+
+    def steps(x, w, gamma):
+        out = []
+        for fmt in ("mxfp4", "mxfp8"):
+            wq, _, ws = s24.mx_quantize(w, "mxfp4", False, True)
+            for rows in (1, 40, 300):
+                q, _, s, _ = s24.mx_rms_norm(x[:rows], gamma, residual=x[:rows], fmt=fmt, want_rows=False, want_tc=True)
+                out.append(s24.mx_matmul(q, s, wq, ws))
+                out.append(s24.mx_dequantize(q, s, layout="tc"))
+        return out
+
+    inputs = [work(1), work(2)]
+    alone = [steps(*i) for i in inputs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(5):
+        together = []
+        for stream, i in zip(streams, inputs):
+            with torch.cuda.stream(stream):
+                together.append(steps(*i))
+        torch.cuda.synchronize()
+        for a, b in zip(alone, together):
+            assert all(torch.equal(x, y) for x, y in zip(a, b))
+    assert s24.lib().s24_device_status(None) == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("fmt", ["mxfp8", "mxfp4"])
+def test_norm_on_exact_borders(s24, fmt, dtype):
+    """rows of +-1 (and +-2): 1 / sqrt(mean + 1e-30) is exactly 1 (a half), so y is the weight itself, which runs through
+    values exactly between two elements and blocks whose largest value is a power of two or one step to its side; zero
+    rows and rows with a single non-zero among them"""
+    k = 4096
+    g = torch.Generator().manual_seed(4)
+    x = torch.where(torch.rand(12, k, generator=g) < 0.5, -1.0, 1.0)
+    x[3] *= 2
+    x[5] = 0
+    x[7] = 0
+    x[7, 100] = 8.0
+    w = torch.ldexp((torch.randint(16, 33, (k,), generator=g) / 16.0 + torch.randint(0, 2, (k,), generator=g) / 32.0),
+                    torch.randint(-9, 1, (k,), generator=g).int())
+    blocks = w.view(-1, 32)
+    blocks[::3, 7] = 2.0
+    blocks[1::3, 7] = 2.0 + torch.finfo(dtype).eps * 2
+    blocks[2::3, 7] = 2.0 - torch.finfo(dtype).eps
+    x, w = x.to(dtype), w.to(dtype)
+    h, y = mxo.rms_norm(x.double().numpy(), None, w.double().numpy(), 1e-30, None)
+    want_c, want_s = mxo.quantize(y, BITS[fmt])
+    codes, scales, _, _ = s24.mx_rms_norm(x.to(DEV), w.to(DEV), eps=1e-30, fmt=fmt)
+    assert np.array_equal(scales.cpu().numpy(), want_s) and np.array_equal(_codes(codes), want_c)
