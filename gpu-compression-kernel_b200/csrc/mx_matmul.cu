@@ -515,6 +515,13 @@ __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t cluster_addr)
     return v;
 }
 
+__device__ __forceinline__ float ld_cluster_f32(uint32_t cluster_addr)
+{
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr));
+    return v;
+}
+
 __device__ __forceinline__ void few_store(const FewParams& p, int i, int j, float v)
 {
     if (i >= p.n_long || j >= p.n_few) return;
@@ -524,8 +531,27 @@ __device__ __forceinline__ void few_store(const FewParams& p, int i, int j, floa
     else static_cast<__half*>(p.C)[at] = __float2half_rn(v);
 }
 
-// This CTA's share of the columns (every S-th), four rows per thread and step: sums of the S partial sums.  The S loads
-// of a step do not wait for one another (one at a time cost 35 us of 75 with 128 rows and S = 2).
+// columns j .. j + 7 of row i of the long side, where they are neighbours in C: 16 bytes at once where they are all there
+// and aligned (3913 x 64 x 256: element by element 11 us, so 3.5)
+__device__ __forceinline__ void few_store_row8(const FewParams& p, int i, int j, const float* v)
+{
+    if (i >= p.n_long || j >= p.n_few) return;
+    const int64_t at = (int64_t)i * p.stride_long + j;
+    if (p.out != S24_FP32 && j + 8 <= p.n_few) {
+        uint16_t* c = static_cast<uint16_t*>(p.C) + at;
+        if ((reinterpret_cast<uintptr_t>(c) & 15u) == 0) {
+            const int bf16 = p.out == S24_BF16;
+            *reinterpret_cast<uint4*>(c) = make_uint4(pack2(v[0], v[1], bf16), pack2(v[2], v[3], bf16), pack2(v[4], v[5], bf16), pack2(v[6], v[7], bf16));
+            return;
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) few_store(p, i, j + k, v[k]);
+}
+
+// This CTA's share of the columns, summed over the S partial sums in the order of the ranks; the S loads of a step do not
+// wait for one another (one at a time cost 35 us of 75 with 128 rows and S = 2).  Where rows of the long side are
+// neighbours in C: every S-th column, four rows per thread and step.
 template <int S>
 __device__ __forceinline__ void few_reduce(const FewParams& p, uint32_t sums, int rank, int row0, int j0, int columns, int thread)
 {
@@ -546,6 +572,32 @@ __device__ __forceinline__ void few_reduce(const FewParams& p, uint32_t sums, in
         few_store(p, row0 + row + 2, j0 + j, v[0].z);
         few_store(p, row0 + row + 3, j0 + j, v[0].w);
     }
+}
+
+// Where the columns are neighbours in C: a row per thread, every S-th eight columns.
+template <int S>
+__device__ __forceinline__ void few_reduce_rows(const FewParams& p, uint32_t sums, int rank, int row0, int j0, int columns, int row)
+{
+    for (int j = 8 * rank; j < columns; j += 8 * S) {
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            float w[S];
+#pragma unroll
+            for (int r = 0; r < S; ++r) w[r] = ld_cluster_f32(mapa(sums + (uint32_t)((j + k) * 128 + row) * 4, (uint32_t)r));
+            v[k] = w[0];
+#pragma unroll
+            for (int r = 1; r < S; ++r) v[k] += w[r];
+        }
+        few_store_row8(p, row0 + row, j0 + j, v);
+    }
+}
+
+template <int S>
+__device__ __forceinline__ void few_reduce_any(const FewParams& p, uint32_t sums, int rank, int row0, int j0, int columns, int thread)
+{
+    if (p.stride_few == 1) few_reduce_rows<S>(p, sums, rank, row0, j0, columns, thread);
+    else few_reduce<S>(p, sums, rank, row0, j0, columns, thread);
 }
 
 template <class Cfg>
@@ -664,7 +716,10 @@ mx_matmul_few_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
                 uint32_t r[16];
                 tc_ld_32x32b_x16(tacc + (uint32_t)c, r);
                 tc_wait_ld();
-                if (split == 1) {
+                if (split == 1 && p.stride_few == 1) {
+                    few_store_row8(p, row0 + row, j0 + c, reinterpret_cast<const float*>(r));
+                    few_store_row8(p, row0 + row, j0 + c + 8, reinterpret_cast<const float*>(r + 8));
+                } else if (split == 1) {
 #pragma unroll
                     for (int j = 0; j < 16; ++j) few_store(p, row0 + row, j0 + c + j, __uint_as_float(r[j]));
                 } else {   // every copy into the stages and every MMA that reads them is done
@@ -683,9 +738,9 @@ mx_matmul_few_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
         cluster_sync();
         if (warp >= 2) {
             const int thread = (int)threadIdx.x - 64;
-            if (split == 2) few_reduce<2>(p, smem_base, rank, row0, j0, columns, thread);
-            else if (split == 4) few_reduce<4>(p, smem_base, rank, row0, j0, columns, thread);
-            else few_reduce<8>(p, smem_base, rank, row0, j0, columns, thread);
+            if (split == 2) few_reduce_any<2>(p, smem_base, rank, row0, j0, columns, thread);
+            else if (split == 4) few_reduce_any<4>(p, smem_base, rank, row0, j0, columns, thread);
+            else few_reduce_any<8>(p, smem_base, rank, row0, j0, columns, thread);
         }
         __syncwarp();
         cluster_sync();   // nobody leaves while another reads its sums
@@ -761,18 +816,6 @@ static int launch_mx(const MxOperand& a, const MxOperand& b, MxParams p, cudaStr
                       "mx_matmul launch");
 }
 
-// K split of the kernel for few rows: as many CTAs as find room at once (two per SM), but a second CTA on an SM only
-// where each still has 8 k-tiles.  Measured, 4-bit weight and 8-bit rows: 32 x 8192 x 8192 18.5 / 13.7 / 12.1 / 17.3 us
-// with 1 / 2 / 4 / 8 CTAs sharing K (64 tiles: 4 fill the SMs), 1 x 4096 x 4096 8.5 / 6.6 / 5.4 / 6.6 (32 tiles: 8 would
-// be a second CTA with 4 k-tiles), 4 x 28672 x 8192 24.3 / 28.8 / 34.7 / 46.8 (224 tiles: 1).
-static int few_split(int tiles, int ktiles)
-{
-    int best = 1;
-    for (int s = 2; s <= 8 && s <= ktiles; s *= 2)
-        if (tiles * s <= sm_count() || (tiles * s <= 2 * sm_count() && ktiles / s >= 8)) best = s;
-    return best;
-}
-
 template <class Cfg>
 static int launch_few(const MxOperand& a, const MxOperand& b, FewParams p, int64_t K, int split, cudaStream_t stream)
 {
@@ -833,33 +876,24 @@ static int run_few(const MxOperand& a, const MxOperand& b, const MxParams& p, in
     return launch_few<FewCfg<F4, 128, 3>>(lng, few, f, p.K, split, stream);
 }
 
-// Which kernel and tile: the least of a time that is a fixed part (launch, first copies, last epilogue) and one per k-tile
-// and pass over the SMs, in microseconds as measured with the operands in L2 at 256 rows and K of 512 to 16384.  What the
-// memory bounds, it bounds for all of them alike.  Measured against it (tiles 256 x 256, 256 x 128, 128 x 128):
-// 256 x 8192 x 8192 4-bit 17.4 / 13.6 / 14.7 us, 512 x 8192 x 8192 8-by-4-bit 28.0 / 30.5 / 34.6, 160 x 1000 x 1024 8-bit
-// 20.5 / 13.7 / 13.1.  K split over a cluster against the best tile: 64 x 28672 x 8192 30.7 / 35.7, 128 x 28672 x 8192
-// 39.1 / 36.7, 129 x 1000 x 16384 12.6 / 27.0, 300 x 1300 x 8192 12.3 / 17.4, 512 x 512 x 4096 7.9 / 6.2.
+// Which kernel and tile: the least of a time model, in microseconds.  A tile costs a fixed part (launch, first copies,
+// last epilogue), one per k-tile and pass over the SMs, and one per further pass; a split of K a fixed part, one per
+// k-tile of a CTA, which doubles where SMs have two, and the sum over the cluster.  The constants are fitted to 150
+// shapes drawn over 1 to 4096 rows, 64 to 16384 columns and K of 256 to 16384 in three pairs of formats, each timed with
+// every tile and split: what the model picks takes 1.02 times the best of them on average, 1.33 at worst.  Examples
+// (tiles 256 x 256, 256 x 128, 128 x 128, then 1, 2, 4, 8 CTAs sharing K): 8192^3 4-bit 185 / 235 / 287 and 341 to 1160 us;
+// 543 x 1792 x 1792 8-by-4-bit 9.6 / 6.6 / 6.2, 12.1 / 12.1 / 10.0 / 20.5; 65 x 561 x 12032 41.8 / 25.0 / 24.4, 36.7 / 22.7 /
+// 13.1 / 8.6; 1 x 4096 x 4096 - / - / 10.0, 7.0 / 5.1 / 4.4 / 5.2; 4 x 28672 x 8192 54 / 74 / 59, 22.3 / 27.1 / 32.8 / 45.
 struct MxPlan {
     double time;
-    int bm, bn, split;   // split > 0: the kernel for few rows
+    int bm, bn, split;   // split > 0: K split over that many CTAs on tiles of at most 128 x 128
 };
-
-static MxPlan plan_few(int64_t few, int64_t lng, int ktiles)
-{
-    const int n = (int)((lng + 127) / 128 * ((few + 127) / 128)), s = few_split(n, ktiles);
-    const double passes = (double)((n * s + 2 * sm_count() - 1) / (2 * sm_count()));
-    const double per_ktile = (few > 64 ? 0.36 : 0.25) * (n * s > sm_count() ? 2.0 : 1.0);
-    return {(few > 64 ? 7.6 : 3.0) + passes * ktiles / s * per_ktile, 0, 0, s};
-}
 
 static MxPlan plan_mx(int64_t M, int64_t N, int ktiles)
 {
-    const int64_t few = M < N ? M : N, lng = M < N ? N : M;
-    // the long side's tiles are the grid's y; K is split where there are fewer tiles than SMs, or few rows
-    const bool few_ok = few <= 128 ? lng <= 65535 * 128 : ((M + 127) / 128) * ((N + 127) / 128) <= sm_count();
-    if (few_ok && few <= 64) return plan_few(few, lng, ktiles);
     struct Tile { int bm, bn, units; double fixed, per_ktile, per_pass; };
-    const Tile tiles[3] = {{256, 256, sm_count() / 2, 5.7, 0.29, 0.0}, {256, 128, sm_count() / 2, 4.7, 0.185, 0.6}, {128, 128, sm_count(), 4.3, 0.21, 0.6}};
+    const int sms = sm_count();
+    const Tile tiles[3] = {{256, 256, sms / 2, 4.2, 0.32, 1.4}, {256, 128, sms / 2, 3.7, 0.18, 1.0}, {128, 128, sms, 3.3, 0.20, 1.1}};
     MxPlan best = {1e30, 0, 0, 0};
     for (const Tile& t : tiles) {
         const int64_t n = ((M + t.bm - 1) / t.bm) * ((N + t.bn - 1) / t.bn);
@@ -867,9 +901,17 @@ static MxPlan plan_mx(int64_t M, int64_t N, int ktiles)
         const double time = t.fixed + passes * ktiles * t.per_ktile + (passes - 1) * t.per_pass;
         if (time < best.time) best = {time, t.bm, t.bn, 0};
     }
-    if (few_ok) {
-        const MxPlan f = plan_few(few, lng, ktiles);
-        if (f.time < best.time) best = f;
+    const int64_t few = M < N ? M : N, lng = M < N ? N : M;
+    if (few <= 8192 && lng <= 65535 * 128) {   // the grid's y and z
+        const double fixed = few <= 16 ? 2.3 : few <= 32 ? 2.6 : few <= 64 ? 2.9 : 5.0;
+        const double per_ktile = few <= 16 ? 0.18 : few <= 32 ? 0.16 : few <= 64 ? 0.20 : 0.26;
+        const double sum = few <= 16 ? 1.1 : few <= 32 ? 1.6 : few <= 64 ? 2.1 : 3.0;
+        const int64_t n = ((lng + 127) / 128) * ((few + 127) / 128);
+        for (int s = 1; s <= 8 && s <= ktiles; s *= 2) {
+            const double passes = (double)((n * s + 2 * sms - 1) / (2 * sms));
+            const double time = fixed + passes * ktiles / s * per_ktile * (n * s > sms ? 2.2 : 1.0) + (s > 1 ? sum : 0.0) + (passes - 1) * 4.0;
+            if (time < best.time) best = {time, 0, 0, s};
+        }
     }
     return best;
 }
