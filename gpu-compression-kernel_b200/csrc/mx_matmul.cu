@@ -880,7 +880,7 @@ static int run_few(const MxOperand& a, const MxOperand& b, const MxParams& p, in
 // last epilogue), one per k-tile and pass over the SMs, and one per further pass; a split of K a fixed part, one per
 // k-tile of a CTA, which doubles where SMs have two, and the sum over the cluster.  The constants are fitted to 150
 // shapes drawn over 1 to 4096 rows, 64 to 16384 columns and K of 256 to 16384 in three pairs of formats, each timed with
-// every tile and split: what the model picks takes 1.02 times the best of them on average, 1.33 at worst.  Examples
+// every tile and split: what the model picks takes 1.014 times the best of them on average, 1.33 at worst.  Examples
 // (tiles 256 x 256, 256 x 128, 128 x 128, then 1, 2, 4, 8 CTAs sharing K): 8192^3 4-bit 185 / 235 / 287 and 341 to 1160 us;
 // 543 x 1792 x 1792 8-by-4-bit 9.6 / 6.6 / 6.2, 12.1 / 12.1 / 10.0 / 20.5; 65 x 561 x 12032 41.8 / 25.0 / 24.4, 36.7 / 22.7 /
 // 13.1 / 8.6; 1 x 4096 x 4096 - / - / 10.0, 7.0 / 5.1 / 4.4 / 5.2; 4 x 28672 x 8192 54 / 74 / 59, 22.3 / 27.1 / 32.8 / 45.
@@ -893,7 +893,7 @@ static MxPlan plan_mx(int64_t M, int64_t N, int ktiles)
 {
     struct Tile { int bm, bn, units; double fixed, per_ktile, per_pass; };
     const int sms = sm_count();
-    const Tile tiles[3] = {{256, 256, sms / 2, 4.2, 0.32, 1.4}, {256, 128, sms / 2, 3.7, 0.18, 1.0}, {128, 128, sms, 3.3, 0.20, 1.1}};
+    const Tile tiles[3] = {{256, 256, sms / 2, 4.2, 0.32, 1.4}, {256, 128, sms / 2, 3.7, 0.195, 1.0}, {128, 128, sms, 3.3, 0.21, 1.1}};
     MxPlan best = {1e30, 0, 0, 0};
     for (const Tile& t : tiles) {
         const int64_t n = ((M + t.bm - 1) / t.bm) * ((N + t.bn - 1) / t.bn);
@@ -906,10 +906,11 @@ static MxPlan plan_mx(int64_t M, int64_t N, int ktiles)
         const double fixed = few <= 16 ? 2.3 : few <= 32 ? 2.6 : few <= 64 ? 2.9 : 5.0;
         const double per_ktile = few <= 16 ? 0.18 : few <= 32 ? 0.16 : few <= 64 ? 0.20 : 0.26;
         const double sum = few <= 16 ? 1.1 : few <= 32 ? 1.6 : few <= 64 ? 2.1 : 3.0;
+        const double second = few <= 64 ? 2.2 : 3.4;   // with a second CTA on an SM (128 columns leave each three stages)
         const int64_t n = ((lng + 127) / 128) * ((few + 127) / 128);
         for (int s = 1; s <= 8 && s <= ktiles; s *= 2) {
             const double passes = (double)((n * s + 2 * sms - 1) / (2 * sms));
-            const double time = fixed + passes * ktiles / s * per_ktile * (n * s > sms ? 2.2 : 1.0) + (s > 1 ? sum : 0.0) + (passes - 1) * 4.0;
+            const double time = fixed + passes * ktiles / s * per_ktile * (n * s > sms ? second : 1.0) + (s > 1 ? sum : 0.0) + (passes - 1) * 4.0;
             if (time < best.time) best = {time, 0, 0, s};
         }
     }
