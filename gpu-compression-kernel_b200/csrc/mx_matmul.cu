@@ -489,23 +489,27 @@ struct FewParams {
 
 constexpr int kFewThreads = 192;   // producer, MMA issuer, four epilogue warps
 
-template <bool F4, int NT, int ST>
+// DEEP: as many stages as one CTA's shared memory holds, where no SM gets a second CTA (128 x 8192 x 28672 57 -> 40 us, one
+// CTA per tile 64 x 8192 x 8192 24 -> 14); otherwise as many as two have room for
+template <bool F4, int NT, bool DEEP>
 struct FewCfg {
     static constexpr bool kF4 = F4;
     static constexpr int kNT = NT;
-    static constexpr int kStages = ST;
     static constexpr int kChunks = F4 ? 2 : 1;
     static constexpr int kABytes = 128 * 128;
     static constexpr int kBBytes = NT * 128;
     static constexpr int kSBytes = kChunks * mx::kRecordBytes;
     static constexpr int kStageBytes = kABytes + kBBytes + 2 * kSBytes;
+    static constexpr int kOtherBytes = 1024 + 256;   // alignment and barriers
+    static constexpr int kFit = ((DEEP ? 232448 : 233472 / 2 - 1024) - kOtherBytes) / kStageBytes;
+    static constexpr int ST = kFit < 12 ? kFit : 12;
+    static constexpr int kStages = ST;
     static constexpr int kScaleCols = 8 * kChunks;
     static constexpr int kScaleCol0 = NT;
     static constexpr int kTmem = NT + kScaleCols <= 32 ? 32 : NT + kScaleCols <= 64 ? 64 : NT + kScaleCols <= 128 ? 128 : 256;
-    static constexpr int kSmemBytes = ST * kStageBytes + 1024 + 128;
+    static constexpr int kSmemBytes = ST * kStageBytes + kOtherBytes;
     static_assert(ST * kStageBytes >= NT * 128 * 4, "the partial sums take the place of the stages");
-    static_assert(8 * (2 * ST + 1) + 16 <= 128, "barrier block");
-    static_assert(2 * (kSmemBytes + 1024) <= 233472, "two CTAs per SM");
+    static_assert(8 * (2 * ST + 1) + 16 <= 256, "barrier block");
 };
 
 __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t cluster_addr)
@@ -816,8 +820,39 @@ static int launch_mx(const MxOperand& a, const MxOperand& b, MxParams p, cudaStr
                       "mx_matmul launch");
 }
 
+// CTAs of the kernel for few rows that the device holds at once with one per SM, in clusters of `split`: fewer than SMs
+// where clusters do not divide the SMs of a GPC (148, 148, 132 and 120 on the device of these measurements)
+static int few_slots(int split)
+{
+    static int cached[64][4] = {};   // each written with the same value, whichever thread gets there first
+    const int log = split == 1 ? 0 : split == 2 ? 1 : split == 4 ? 2 : 3;
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return sm_count();
+    int& slots = cached[dev][log];
+    if (slots == 0) {
+        using Cfg = FewCfg<false, 16, true>;
+        cudaLaunchConfig_t lc = {};
+        lc.gridDim = dim3((unsigned)split, 1024);
+        lc.blockDim = dim3(kFewThreads);
+        lc.dynamicSmemBytes = Cfg::kSmemBytes;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = (unsigned)split;
+        attr[0].val.clusterDim.y = 1;
+        attr[0].val.clusterDim.z = 1;
+        lc.attrs = attr;
+        lc.numAttrs = 1;
+        int n = 0;
+        if (cudaFuncSetAttribute(mx_matmul_few_kernel<Cfg>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes) != cudaSuccess ||
+            cudaOccupancyMaxActiveClusters(&n, mx_matmul_few_kernel<Cfg>, &lc) != cudaSuccess)
+            cudaGetLastError();
+        slots = n > 0 ? n * split : sm_count();
+    }
+    return slots;
+}
+
 template <class Cfg>
-static int launch_few(const MxOperand& a, const MxOperand& b, FewParams p, int64_t K, int split, cudaStream_t stream)
+static int launch_few_cfg(const MxOperand& a, const MxOperand& b, FewParams p, int64_t K, int split, cudaStream_t stream)
 {
     CUtensorMap tm_a, tm_b, tm_sa, tm_sb;
     int rc = make_code_map(&tm_a, a, K, Cfg::kF4, 128, "codes of the long side");
@@ -826,7 +861,6 @@ static int launch_few(const MxOperand& a, const MxOperand& b, FewParams p, int64
     if (!rc) rc = make_scale_map(&tm_sb, b, K, Cfg::kChunks, 1, "scales of the few rows");
     if (rc) return rc;
     p.tx_bytes = code_tx(a, Cfg::kF4, 128) + code_tx(b, Cfg::kF4, Cfg::kNT) + 2 * Cfg::kSBytes;
-    p.ktiles = (int)((K + 128 * Cfg::kChunks - 1) / (128 * Cfg::kChunks));
     {
         static bool opted_in[64] = {false};
         int dev = 0;
@@ -840,10 +874,19 @@ static int launch_few(const MxOperand& a, const MxOperand& b, FewParams p, int64
         }
     }
     const int tiles = (p.n_long + 127) / 128, across = (p.n_few + Cfg::kNT - 1) / Cfg::kNT;
-    if (split > p.ktiles) split = 1;
     return check_cuda(mx::launch_overlapped(mx_matmul_few_kernel<Cfg>, dim3((unsigned)split, (unsigned)tiles, (unsigned)across), kFewThreads, Cfg::kSmemBytes, (unsigned)split, stream,
                                             tm_a, tm_b, tm_sa, tm_sb, p),
                       "mx_matmul launch");
+}
+
+template <bool F4, int NT>
+static int launch_few(const MxOperand& a, const MxOperand& b, FewParams p, int64_t K, int split, cudaStream_t stream)
+{
+    p.ktiles = (int)((K + (F4 ? 255 : 127)) / (F4 ? 256 : 128));
+    if (split > p.ktiles) split = 1;
+    const int64_t ctas = (int64_t)((p.n_long + 127) / 128) * ((p.n_few + NT - 1) / NT) * split;
+    if (ctas <= few_slots(split)) return launch_few_cfg<FewCfg<F4, NT, true>>(a, b, p, K, split, stream);
+    return launch_few_cfg<FewCfg<F4, NT, false>>(a, b, p, K, split, stream);
 }
 
 template <bool F4>
@@ -866,24 +909,22 @@ static int run_few(const MxOperand& a, const MxOperand& b, const MxParams& p, in
     f.tx_bytes = 0;
     f.status = p.status;
     f.wait_limit_ns = p.wait_limit_ns;
-    if constexpr (!F4) {
-        // eight columns leave room for a sixth stage: 4 x 28672 x 8192 with a 4-bit weight 23.0 -> 22.3 us
-        if (f.n_few <= 8) return launch_few<FewCfg<F4, 8, 6>>(lng, few, f, p.K, split, stream);
-    }
-    if (f.n_few <= 16) return launch_few<FewCfg<F4, 16, 5>>(lng, few, f, p.K, split, stream);
-    if (f.n_few <= 32) return launch_few<FewCfg<F4, 32, 5>>(lng, few, f, p.K, split, stream);
-    if (f.n_few <= 64) return launch_few<FewCfg<F4, 64, 4>>(lng, few, f, p.K, split, stream);
-    return launch_few<FewCfg<F4, 128, 3>>(lng, few, f, p.K, split, stream);
+    // eight columns leave room for a sixth stage beside 8-bit rows: 4 x 28672 x 8192 with a 4-bit weight 23.0 -> 22.3 us
+    if (f.n_few <= 8) return launch_few<F4, 8>(lng, few, f, p.K, split, stream);
+    if (f.n_few <= 16) return launch_few<F4, 16>(lng, few, f, p.K, split, stream);
+    if (f.n_few <= 32) return launch_few<F4, 32>(lng, few, f, p.K, split, stream);
+    if (f.n_few <= 64) return launch_few<F4, 64>(lng, few, f, p.K, split, stream);
+    return launch_few<F4, 128>(lng, few, f, p.K, split, stream);
 }
 
 // Which kernel and tile: the least of a time model, in microseconds.  A tile costs a fixed part (launch, first copies,
 // last epilogue), one per k-tile and pass over the SMs, and one per further pass; a split of K a fixed part, one per
-// k-tile of a CTA, which doubles where SMs have two, and the sum over the cluster.  The constants are fitted to 150
-// shapes drawn over 1 to 4096 rows, 64 to 16384 columns and K of 256 to 16384 in three pairs of formats, each timed with
-// every tile and split: what the model picks takes 1.014 times the best of them on average, 1.33 at worst.  Examples
+// k-tile of a CTA, more where SMs have two, and the sum over the cluster.  The constants are fitted to 220 shapes drawn
+// over 1 to 4096 rows, 64 to 16384 columns and K of 256 to 16384 in three pairs of formats, each timed with every tile and
+// split; on 218 others what the model picks takes 1.02 times the best of them on average, 1.24 at worst.  Examples
 // (tiles 256 x 256, 256 x 128, 128 x 128, then 1, 2, 4, 8 CTAs sharing K): 8192^3 4-bit 185 / 235 / 287 and 341 to 1160 us;
 // 543 x 1792 x 1792 8-by-4-bit 9.6 / 6.6 / 6.2, 12.1 / 12.1 / 10.0 / 20.5; 65 x 561 x 12032 41.8 / 25.0 / 24.4, 36.7 / 22.7 /
-// 13.1 / 8.6; 1 x 4096 x 4096 - / - / 10.0, 7.0 / 5.1 / 4.4 / 5.2; 4 x 28672 x 8192 54 / 74 / 59, 22.3 / 27.1 / 32.8 / 45.
+// 13.1 / 8.6; 1 x 4096 x 4096 15 / 16 / 10, 7.0 / 5.2 / 4.6 / 5.2; 4 x 28672 x 8192 54 / 74 / 59, 22.2 / 27.4 / 32.9 / 45.
 struct MxPlan {
     double time;
     int bm, bn, split;   // split > 0: K split over that many CTAs on tiles of at most 128 x 128
@@ -893,7 +934,7 @@ static MxPlan plan_mx(int64_t M, int64_t N, int ktiles)
 {
     struct Tile { int bm, bn, units; double fixed, per_ktile, per_pass; };
     const int sms = sm_count();
-    const Tile tiles[3] = {{256, 256, sms / 2, 4.2, 0.32, 1.4}, {256, 128, sms / 2, 3.7, 0.195, 1.0}, {128, 128, sms, 3.3, 0.21, 1.1}};
+    const Tile tiles[3] = {{256, 256, sms / 2, 4.3, 0.31, 2.0}, {256, 128, sms / 2, 3.7, 0.19, 1.2}, {128, 128, sms, 3.2, 0.21, 1.1}};
     MxPlan best = {1e30, 0, 0, 0};
     for (const Tile& t : tiles) {
         const int64_t n = ((M + t.bm - 1) / t.bm) * ((N + t.bn - 1) / t.bn);
@@ -903,14 +944,14 @@ static MxPlan plan_mx(int64_t M, int64_t N, int ktiles)
     }
     const int64_t few = M < N ? M : N, lng = M < N ? N : M;
     if (few <= 8192 && lng <= 65535 * 128) {   // the grid's y and z
-        const double fixed = few <= 16 ? 2.3 : few <= 32 ? 2.6 : few <= 64 ? 2.9 : 5.0;
-        const double per_ktile = few <= 16 ? 0.18 : few <= 32 ? 0.16 : few <= 64 ? 0.20 : 0.26;
-        const double sum = few <= 16 ? 1.1 : few <= 32 ? 1.6 : few <= 64 ? 2.1 : 3.0;
-        const double second = few <= 64 ? 2.2 : 3.4;   // with a second CTA on an SM (128 columns leave each three stages)
+        const double fixed = few <= 16 ? 2.4 : few <= 32 ? 2.7 : few <= 64 ? 3.0 : 4.9;
+        const double per_ktile = few <= 64 ? 0.15 : 0.20;
+        const double sum = few <= 16 ? 1.1 : few <= 32 ? 1.7 : few <= 64 ? 2.2 : 3.0;
+        const double second = few <= 64 ? 2.6 : 3.2;   // with a second CTA on an SM and half the stages for each
         const int64_t n = ((lng + 127) / 128) * ((few + 127) / 128);
         for (int s = 1; s <= 8 && s <= ktiles; s *= 2) {
-            const double passes = (double)((n * s + 2 * sms - 1) / (2 * sms));
-            const double time = fixed + passes * ktiles / s * per_ktile * (n * s > sms ? second : 1.0) + (s > 1 ? sum : 0.0) + (passes - 1) * 4.0;
+            const double passes = (double)((n * s + 2 * few_slots(s) - 1) / (2 * few_slots(s)));
+            const double time = fixed + passes * ktiles / s * per_ktile * (n * s > few_slots(s) ? second : 1.0) + (s > 1 ? sum : 0.0) + (passes - 1) * 4.0;
             if (time < best.time) best = {time, 0, 0, s};
         }
     }
