@@ -472,9 +472,10 @@ mx_matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
 //
 // With few rows on one side (a decoding step) the product is the reading of the other side's codes.  That side
 // ("long") takes the 128 rows of the MMA, the few rows its NT columns, and K is split over the S CTAs of a cluster so
-// that all SMs read; a product of any size that has too few 128 x 128 tiles for the SMs is split the same way.  Each CTA multiplies its share of the k-tiles, leaves its partial sums (fp32) in its shared
-// memory, and each then adds 1 / S of the columns over the S CTAs, in the order of their ranks, and stores them.
-// No workspace, no atomics, one launch, the same sums whatever order the CTAs run in.
+// that all SMs read; a product of any size that has too few 128 x 128 tiles for the SMs is split the same way.  Each
+// CTA multiplies its share of the k-tiles, leaves its partial sums (fp32) in its shared memory, and each then adds 1 / S
+// of the columns over the S CTAs, in the order of their ranks, and stores them.  No workspace, no atomics, one launch,
+// the same sums whatever order the CTAs run in.
 
 struct FewParams {
     void* C;
@@ -515,14 +516,14 @@ struct FewCfg {
 __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t cluster_addr)
 {
     float4 v;
-    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(cluster_addr));
+    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(cluster_addr) : "memory");
     return v;
 }
 
 __device__ __forceinline__ float ld_cluster_f32(uint32_t cluster_addr)
 {
     float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr) : "memory");
     return v;
 }
 
