@@ -9,9 +9,10 @@
  * set-up and debug helpers and say so: s24_peer_alloc / s24_peer_free / s24_peer_open /
  * s24_peer_close (multi-GPU buffers) and s24_device_status (reads a status word back).
  *
- * Per-device state.  The library caches three things per device ordinal, each written once
+ * Per-device state.  The library caches four things per device ordinal, each written once
  * with the same value whichever thread gets there first (so concurrent first calls are
- * benign, but the caches are not locked): the SM count, the large-shared-memory opt-in of
+ * benign, but the caches are not locked): the SM count, how many clusters of each size the
+ * device holds at once (s24_mx_matmul), the large-shared-memory opt-in of
  * each GEMM variant, and the device addresses of two objects inside the library image (the
  * status word and the built-in scratch buffer, looked up with cudaGetSymbolAddress).  They
  * assume one CUDA context per device for the life of the process (the primary context that
