@@ -97,8 +97,10 @@ struct MxParams {
     int M, N, K;
     int out;                 // S24_FP16 / S24_BF16 / S24_FP32
     uint32_t a_format, b_format;
-    uint32_t tx_bytes;       // bytes a CTA's copies of one k-tile deliver
+    uint32_t tx_bytes;       // bytes a CTA's copies of one k-tile deliver, B's codes aside
+    uint32_t tx_box;         // and each box of B's codes
     int wide;                // rows of C allow 32-byte stores
+    int whole, steps;        // mx_tile
     int* status;
     unsigned long long wait_limit_ns;
 };
@@ -106,19 +108,38 @@ struct MxParams {
 constexpr int kStorePitch = 33;                              // words: 32 of a row and one against bank conflicts
 constexpr int kStoreWarpBytes = 32 * kStorePitch * 4;
 
-// Tile t of the persistent walk: groups of 16 row tiles swept along N.  Of groups of 4 / 8 / 16 / 32, seconds under load:
+// Output tiles in groups of 16 row tiles swept along N.  Of groups of 4 / 8 / 16 / 32, seconds under load:
 // 8192^3 4-bit 210 / 210 / 208 / 207 us, 8-bit 438 / 428 / 421 / 468, 4001 x 28672 x 8192 700 / 689 / 682 / 682,
 // 16384^3 4-bit 1639 / 1577 / 1550 / 1746.
 constexpr int kMxGroupM = 16;
-__device__ __forceinline__ void mx_tile_coords(int t, int num_m, int num_n, int& tm, int& tn)
+constexpr int kMxPart = 128;   // a tile's columns start on a record of B's scales
+
+struct MxTile {
+    int m, col, width;   // row tile, first column, columns the MMA makes: a multiple of 64; none: nothing left to do
+};
+
+// Step t of the persistent walk.  The tiles of a last pass that leaves half of the units idle, those from p.whole on, are
+// two steps of 128 columns each, and a tile that N ends in is as narrow as it can be (1537 x 6150 x 4128 8-bit 41.2 -> 38.4
+// us, 2000 x 10000 x 4096 8-by-4-bit 60.1 -> 57.6, 2560 x 2048 x 4096 4-bit 15.1 -> 13.2).
+template <int BN>
+__device__ __forceinline__ MxTile mx_tile(const MxParams& p, int t, int num_m, int num_n)
 {
+    int part = 0, columns = BN;
+    if (BN > kMxPart && t >= p.whole) {
+        part = (t - p.whole) & 1;
+        t = p.whole + ((t - p.whole) >> 1);
+        columns = kMxPart;
+    }
     const int group_size = kMxGroupM * num_n;
     const int group = t / group_size;
     const int first_m = group * kMxGroupM;
     const int gm = min(num_m - first_m, kMxGroupM);
     const int in_group = t - group * group_size;
-    tm = first_m + in_group % gm;
-    tn = in_group / gm;
+    MxTile tile;
+    tile.m = first_m + in_group % gm;
+    tile.col = in_group / gm * BN + part * kMxPart;
+    tile.width = min(columns, (p.N - tile.col + 63) / 64 * 64);
+    return tile;
 }
 
 // ALIGNED: rows of C start on 32 bytes; otherwise a stage of the ring makes room for the stores' staging
@@ -132,6 +153,9 @@ struct MxCfg {
     static constexpr int kKTile = F4 ? 256 : 128;               // elements of K: 128 bytes of a row
     static constexpr int kChunks = kKTile / 128;                // scale records per 128 rows
     static constexpr int kBNCta = BN / G;
+    // rows of B in one copy: a tile's half is copied alone (an SM takes in 64 bytes a cycle, so an MMA half as wide is no
+    // faster where the rows of a whole one come with it), and whole tiles run 2 to 3 % faster with two copies as well
+    static constexpr int kBox = kBNCta < kMxPart / G ? kBNCta : kMxPart / G;
     static constexpr int kTilesB = (BN + 127) / 128;            // record rows of B's scales
     static constexpr int kABytes = 128 * 128;
     static constexpr int kBBytes = kBNCta * 128;
@@ -292,7 +316,6 @@ mx_matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
 
     const int num_m = (p.M + 128 * G - 1) / (128 * G);
     const int num_n = (p.N + BN - 1) / BN;
-    const int num_tiles = num_m * num_n;
     const int num_units = (int)gridDim.x / G;
     const int unit = (int)blockIdx.x / G;
     const int ktiles = (p.K + Cfg::kKTile - 1) / Cfg::kKTile;   // elements and scales beyond K read as zeros
@@ -333,11 +356,13 @@ mx_matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
             bool stopped = false;
             // 4-bit operands of kind::mxf4 are copied as bytes, two elements each; the others by element
             constexpr int kStep = 128;
-            for (int t = unit; t < num_tiles && !stopped && !*abort_flag; t += num_units) {
-                int tm, tn;
-                mx_tile_coords(t, num_m, num_n, tm, tn);
-                const int row0 = (tm * G + (int)cta_rank) * 128;
-                const int col0 = tn * BN + (int)cta_rank * Cfg::kBNCta;
+            for (int t = unit; t < p.steps && !stopped && !*abort_flag; t += num_units) {
+                const MxTile tile = mx_tile<BN>(p, t, num_m, num_n);
+                if (tile.width <= 0) break;   // the second half of a narrow tile: a unit's last step
+                const int row0 = (tile.m * G + (int)cta_rank) * 128;
+                const int col0 = tile.col + (int)cta_rank * (tile.width / G);
+                const int boxes = Cfg::kBNCta > Cfg::kBox && tile.width > kMxPart ? 2 : 1;
+                const uint32_t tx_bytes = G * (p.tx_bytes + (uint32_t)boxes * p.tx_box);
                 for (int kt = 0; kt < ktiles; ++kt) {
                     if (!mbar_wait(bar_empty + 8 * s, ph ^ 1u, p.wait_limit_ns)) {
                         report_timeout(p.status, abort_flag, 1);
@@ -345,11 +370,12 @@ mx_matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
                         break;
                     }
                     const uint32_t full = (G == 2) ? mapa(bar_full + 8 * s, 0) : (bar_full + 8 * s);
-                    if (leader) mbar_arrive_expect_tx(bar_full + 8 * s, G * p.tx_bytes);
+                    if (leader) mbar_arrive_expect_tx(bar_full + 8 * s, tx_bytes);
                     tma_load_rows<G>(smem_a + s * Cfg::kABytes, &tm_a, kt * kStep, row0, full);
                     tma_load_rows<G>(smem_b + s * Cfg::kBBytes, &tm_b, kt * kStep, col0, full);
+                    if (boxes > 1) tma_load_rows<G>(smem_b + s * Cfg::kBBytes + Cfg::kBox * 128, &tm_b, kt * kStep, col0 + Cfg::kBox, full);
                     tma_load_3d<G>(smem_sa + s * Cfg::kSABytes, &tm_sa, 0, kt * Cfg::kChunks, row0 / 128, full);
-                    tma_load_3d<G>(smem_sb + s * Cfg::kSBBytes, &tm_sb, 0, kt * Cfg::kChunks, tn * BN / 128, full);
+                    tma_load_3d<G>(smem_sb + s * Cfg::kSBBytes, &tm_sb, 0, kt * Cfg::kChunks, tile.col / 128, full);
                     if (++s == ST) { s = 0; ph ^= 1u; }
                 }
             }
@@ -357,13 +383,15 @@ mx_matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
     } else if (warp == 1) {
         // ------------------------------------------------------------ MMA issuer (leader CTA only)
         if (leader && elect_one()) {
-            const uint32_t idesc = make_idesc_scaled(p.a_format, p.b_format, 128 * G, BN);
             const uint32_t sfa = tmem_base + (uint32_t)Cfg::kScaleCol0;
             const uint32_t sfb = sfa + 4 * Cfg::kChunks;
             int s = 0, n = 0;   // n: tiles done
             uint32_t ph = 0;
             bool ok = true;
-            for (int t = unit; t < num_tiles && ok && !*abort_flag; t += num_units, ++n) {
+            for (int t = unit; t < p.steps && ok && !*abort_flag; t += num_units, ++n) {
+                const int width = mx_tile<BN>(p, t, num_m, num_n).width;
+                if (width <= 0) break;
+                const uint32_t idesc = make_idesc_scaled(p.a_format, p.b_format, 128 * G, width);
                 const uint32_t tmem_d = tmem_base + (uint32_t)((n & 1) * Cfg::kAccStep);
                 for (int kt = 0; kt < ktiles; ++kt) {
                     if (!mbar_wait(bar_full + 8 * s, ph, p.wait_limit_ns)) {
@@ -413,21 +441,21 @@ mx_matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
         // ------------------------------------------------------------ epilogue warps
         const int quad = warp & 3;
         const int half = (warp - 2) >> 2;
-        constexpr int CW = BN / 2;
         const uint32_t staging = Cfg::kAligned ? 0u : smem_store + (uint32_t)(warp - 2) * kStoreWarpBytes;
         const uint32_t acc_empty = (G == 2) ? mapa(bar_acc_empty, 0) : bar_acc_empty;
         int n = 0;
-        for (int t = unit; t < num_tiles && !*abort_flag; t += num_units, ++n) {
-            int tm, tn;
-            mx_tile_coords(t, num_m, num_n, tm, tn);
+        for (int t = unit; t < p.steps && !*abort_flag; t += num_units, ++n) {
+            const MxTile tile = mx_tile<BN>(p, t, num_m, num_n);
+            if (tile.width <= 0) break;
+            const int cw = BN > 128 && tile.width > 128 ? 128 : 64;   // columns of a warp
             if (!__all_sync(0xFFFFFFFFu, mbar_wait(bar_acc_full, (uint32_t)n & 1u, p.wait_limit_ns))) {
                 if (lane == 0) report_timeout(p.status, abort_flag, 4);
                 break;
             }
             tc_fence_after();
-            const uint32_t tacc = tmem_base + (uint32_t)((n & 1) * Cfg::kAccStep + half * CW) + ((uint32_t)(32 * quad) << 16);
-            const int row0 = (tm * G + (int)cta_rank) * 128 + 32 * quad;
-            const int col = tn * BN + half * CW;
+            const uint32_t tacc = tmem_base + (uint32_t)((n & 1) * Cfg::kAccStep + half * cw) + ((uint32_t)(32 * quad) << 16);
+            const int row0 = (tile.m * G + (int)cta_rank) * 128 + 32 * quad;
+            const int col = tile.col + half * cw;
             // The 32 columns that both accumulators cover are the first's last ones and the second's first ones: the warp
             // that owns them reads its 64 columns with them first and hands them back; every warp arrives, whether it has a
             // share or not.
@@ -438,8 +466,8 @@ mx_matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
                 if (lane == 0) mbar_arrive_remote(acc_empty);
             }
 #pragma unroll 1
-            for (int i = 0; i < CW / 64; ++i) {
-                const int c = (n & 1) ? 64 * i : CW - 64 - 64 * i;
+            for (int i = 0; i < cw / 64; ++i) {
+                const int c = (n & 1) ? 64 * i : cw - 64 - 64 * i;
                 uint32_t r[64];
                 tc_ld_32x32b_x64(tacc + (uint32_t)c, r);
                 tc_wait_ld();
@@ -448,7 +476,7 @@ mx_matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
                     __syncwarp();
                     if (lane == 0) mbar_arrive_remote(acc_empty);
                 }
-                if (row0 < p.M && col + c < p.N) {   // the same for the whole warp
+                if (row0 < p.M && half * cw + c < tile.width) {   // the same for the whole warp
                     if constexpr (Cfg::kAligned) mx_store_aligned(p, row0, col + c, r, lane);
                     else mx_store_any(p, row0, col + c, r, staging, lane);
                 }
@@ -795,11 +823,12 @@ static int launch_mx(const MxOperand& a, const MxOperand& b, MxParams p, cudaStr
 {
     CUtensorMap tm_a, tm_b, tm_sa, tm_sb;
     int rc = make_code_map(&tm_a, a, p.K, Cfg::kF4, 128, "A codes");
-    if (!rc) rc = make_code_map(&tm_b, b, p.K, Cfg::kF4, Cfg::kBNCta, "B codes");
+    if (!rc) rc = make_code_map(&tm_b, b, p.K, Cfg::kF4, Cfg::kBox, "B codes");
     if (!rc) rc = make_scale_map(&tm_sa, a, p.K, Cfg::kChunks, 1, "A scales");
     if (!rc) rc = make_scale_map(&tm_sb, b, p.K, Cfg::kChunks, Cfg::kTilesB, "B scales");
     if (rc) return rc;
-    p.tx_bytes = code_tx(a, Cfg::kF4, 128) + code_tx(b, Cfg::kF4, Cfg::kBNCta) + Cfg::kSABytes + Cfg::kSBBytes;
+    p.tx_bytes = code_tx(a, Cfg::kF4, 128) + Cfg::kSABytes + Cfg::kSBBytes;
+    p.tx_box = code_tx(b, Cfg::kF4, Cfg::kBox);
     {
         static bool opted_in[64] = {false};
         int dev = 0;
@@ -816,6 +845,10 @@ static int launch_mx(const MxOperand& a, const MxOperand& b, MxParams p, cudaStr
     if (tiles > 0x7FFFFFFFll / kMxGroupM) return fail(S24_ERR_SHAPE, "mx_matmul: too many output tiles");
     int units = sm_count() / Cfg::kG;
     if (units > tiles) units = (int)tiles;
+    // a last pass for at most half of the units: each tile's halves to two of them
+    const int last = (int)(tiles % units);
+    p.whole = (int)(Cfg::kBN > kMxPart && tiles > units && 2 * last <= units ? tiles - last : tiles);
+    p.steps = p.whole + 2 * (int)(tiles - p.whole);
     return check_cuda(mx::launch_overlapped(mx_matmul_kernel<Cfg>, dim3((unsigned)(units * Cfg::kG)), kMxThreads, Cfg::kSmemBytes, Cfg::kG, stream, tm_a, tm_b,
                                             tm_sa, tm_sb, p),
                       "mx_matmul launch");
@@ -939,7 +972,9 @@ static MxPlan plan_mx(int64_t M, int64_t N, int ktiles)
     MxPlan best = {1e30, 0, 0, 0};
     for (const Tile& t : tiles) {
         const int64_t n = ((M + t.bm - 1) / t.bm) * ((N + t.bn - 1) / t.bn);
-        const double passes = (double)((n + t.units - 1) / t.units);
+        // a last pass in halves costs two thirds of one
+        const int64_t last = n % t.units;
+        const double passes = (double)(n / t.units) + (last == 0 ? 0.0 : t.bn > kMxPart && n > t.units && 2 * last <= t.units ? 0.67 : 1.0);
         const double time = t.fixed + passes * ktiles * t.per_ktile + (passes - 1) * t.per_pass;
         if (time < best.time) best = {time, t.bm, t.bn, 0};
     }
@@ -1032,8 +1067,9 @@ extern "C" int s24_mx_matmul(const void* a, const void* a_scales, const void* b,
     p.out = out_dtype;
     p.a_format = both4 ? 1u : fmt_a == S24_MXFP4 ? 5u : 0u;
     p.b_format = both4 ? 1u : fmt_b == S24_MXFP4 ? 5u : 0u;
-    p.tx_bytes = 0;
+    p.tx_bytes = p.tx_box = 0;
     p.wide = aligned(C, 32) && (ldc * esz) % 32 == 0;
+    p.whole = p.steps = 0;
     p.status = status;
     p.wait_limit_ns = kWaitTimeoutNs;
     const MxOperand oa = {a, a_scales, M, lda, fmt_a}, ob = {b, b_scales, N, ldb, fmt_b};

@@ -240,6 +240,22 @@ def test_product_is_exact_where_sums_are(s24, m, n, k, fa, fb):
 
 
 @pytest.mark.parametrize("fa,fb", PAIRS)
+@pytest.mark.parametrize("m,n,k", [(2560, 2050, 256), (2560, 2178, 384), (5000, 1040, 512), (4100, 1281, 256), (300, 11000, 512), (2500, 2700, 128)])
+def test_product_whose_last_pass_is_shared(s24, m, n, k, fa, fb):
+    """some more tiles than the device has SM pairs, in a window of a wider result that keeps what surrounds it"""
+    a, sa, va = _operand(s24, m, k, fa, 1000 * m + k, True)
+    b, sb, vb = _operand(s24, n, k, fb, 1000 * n + k + 1, True)
+    want = (torch.from_numpy(va).to(DEV) @ torch.from_numpy(vb).to(DEV).t()).float()
+    for left, width in ((0, n), (32, -(-n // 32) * 32 + 96), (3, n + 8)):
+        for tile in (None, {"BM": 256, "BN": 256}, {"BM": 256, "BN": 128}):
+            full = torch.full((m + 2, width), 7.0, dtype=torch.float32, device=DEV)
+            s24.mx_matmul(a, sa, b, sb, out_dtype=torch.float32, out=full[1:m + 1, left:left + n], manual_config=tile)
+            assert torch.equal(full[1:m + 1, left:left + n], want), f"tile {tile}"
+            full[1:m + 1, left:left + n] = 7.0
+            assert bool((full == 7.0).all()), f"tile {tile}: written outside"
+
+
+@pytest.mark.parametrize("fa,fb", PAIRS)
 @pytest.mark.parametrize("m,n,k", [(5, 300, 4096), (300, 700, 2048), (64, 256, 16384), (1030, 520, 8192)])
 def test_product_of_quantized_data(s24, m, n, k, fa, fb):
     a, sa, va = _operand(s24, m, k, fa, m + k, False)
