@@ -11,7 +11,8 @@
 //   * warp 0: TMA producer, one ring of k-tiles (A rows, B rows, and the scale records of both);
 //   * warp 1: MMA issuer.  Per k-tile tcgen05.cp brings the scale records into tensor memory (each 512-byte
 //     record is 32 lanes x 4 columns, copied to all four lane quadrants), then four MMAs;
-//   * warps 2-9: epilogue, two per 32-lane quadrant, each half of the tile's columns.
+//   * warps 2-9: epilogue, two per 32-lane quadrant, 64 of the tile's columns each in turn (with a half of the tile for
+//     each the sectors that unaligned rows share were written further apart: 4078 x 13733 x 384 55 us, so 50).
 // In a pair each CTA holds its own 128 rows of A and half of the rows of B, but the scales of all rows of B.
 // Every wait is bounded as in the sparse GEMM (s24_device_status).
 #include "mx_common.cuh"
@@ -447,15 +448,14 @@ mx_matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
         for (int t = unit; t < p.steps && !*abort_flag; t += num_units, ++n) {
             const MxTile tile = mx_tile<BN>(p, t, num_m, num_n);
             if (tile.width <= 0) break;
-            const int cw = BN > 128 && tile.width > 128 ? 128 : 64;   // columns of a warp
+            const int turns = BN > 128 && tile.width > 128 ? 2 : 1;
             if (!__all_sync(0xFFFFFFFFu, mbar_wait(bar_acc_full, (uint32_t)n & 1u, p.wait_limit_ns))) {
                 if (lane == 0) report_timeout(p.status, abort_flag, 4);
                 break;
             }
             tc_fence_after();
-            const uint32_t tacc = tmem_base + (uint32_t)((n & 1) * Cfg::kAccStep + half * cw) + ((uint32_t)(32 * quad) << 16);
+            const uint32_t tacc = tmem_base + (uint32_t)((n & 1) * Cfg::kAccStep) + ((uint32_t)(32 * quad) << 16);
             const int row0 = (tile.m * G + (int)cta_rank) * 128 + 32 * quad;
-            const int col = tile.col + half * cw;
             // The 32 columns that both accumulators cover are the first's last ones and the second's first ones: the warp
             // that owns them reads its 64 columns with them first and hands them back; every warp arrives, whether it has a
             // share or not.
@@ -466,8 +466,8 @@ mx_matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
                 if (lane == 0) mbar_arrive_remote(acc_empty);
             }
 #pragma unroll 1
-            for (int i = 0; i < cw / 64; ++i) {
-                const int c = (n & 1) ? 64 * i : cw - 64 - 64 * i;
+            for (int i = 0; i < turns; ++i) {
+                const int c = 128 * ((n & 1) ? i : turns - 1 - i) + 64 * half;
                 uint32_t r[64];
                 tc_ld_32x32b_x64(tacc + (uint32_t)c, r);
                 tc_wait_ld();
@@ -476,9 +476,9 @@ mx_matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
                     __syncwarp();
                     if (lane == 0) mbar_arrive_remote(acc_empty);
                 }
-                if (row0 < p.M && half * cw + c < tile.width) {   // the same for the whole warp
-                    if constexpr (Cfg::kAligned) mx_store_aligned(p, row0, col + c, r, lane);
-                    else mx_store_any(p, row0, col + c, r, staging, lane);
+                if (row0 < p.M && c < tile.width) {   // the same for the whole warp
+                    if constexpr (Cfg::kAligned) mx_store_aligned(p, row0, tile.col + c, r, lane);
+                    else mx_store_any(p, row0, tile.col + c, r, staging, lane);
                 }
                 __syncwarp();
             }
