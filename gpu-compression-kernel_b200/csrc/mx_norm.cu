@@ -2,44 +2,44 @@
 //
 //   h = round(x + residual)   (or x),   y = h * w / sqrt(mean(h^2) + eps),   (codes, scales) = quantise(y)
 //
-// y is never rounded to 16 bits in between, and codes and scales are those of the formula in 64 bits: a
-// rounding to 8 or 4 bits turns the last bit of y into a whole step of the format wherever y lies at a
-// border, so near one y is carried further than fp32.
+// y is never rounded to 16 bits in between, and codes and scales are those of the formula in 64 bits,
+// h / sqrt(sum(h^2) / K + eps) * w with each operation rounded to fp64: a rounding to 8 or 4 bits turns the
+// last bit of y into a whole step of the format wherever y lies at a border, so near one y is computed in
+// fp64.
 //   * the sum of squares is held in fp64 (squares of 16-bit values are exact there), in a fixed order;
-//   * 1 / sqrt(.) is computed once per row in fp64 and used as a sum of two fp32 numbers;
+//   * 1 / sqrt(.) is computed once per row in fp64 and rounded to fp32;
 //   * y is first computed in fp32 (off by at most 2.5 * 2^-24 of itself) and rounded to the element type
 //     from both ends of y * (1 +- 2^-21): where the two agree, the code is certain.  About one element in
-//     10^5 lies nearer to a border; its thread computes y again with the rounding error of each product
-//     kept (one fused multiply-add) and rounds it to odd: an inexact y gets its last bit set, so the one
-//     rounding to the element type sees on which side of the border y lies (rounding to odd, then to
-//     nearest with at least two bits fewer, is a single rounding).
-// Values of y beyond the fp32 range count as infinite.
+//     10^5 lies nearer to a border; its thread computes y again, in fp64 as the formula reads (a root and a
+//     division: a value that the formula puts exactly on a border stays there), and rounds it to fp32 to
+//     odd: an inexact y gets its last bit set, so the one rounding to the element type sees on which side
+//     of the border y lies (rounding to odd, then to nearest with at least two bits fewer, is a single
+//     rounding).
+// Values of y from 2^128 on count as infinite.
 #include "mx_common.cuh"
 
 namespace s24 {
 
 using namespace mx;
 
-// value + error, where value is the nearest fp32 number to the sum, rounded to odd
-__device__ __forceinline__ float round_to_odd(float value, float error)
+// y in fp32, rounded to odd: towards zero, and the last bit set if that dropped anything
+__device__ __forceinline__ float round_to_odd(double y)
 {
-    const uint32_t b = __float_as_uint(value), e = __float_as_uint(error);
-    const uint32_t exponent = b & 0x7F800000u;
-    // even and inexact: the odd neighbour towards the exact value
-    if (error != 0.0f && !(b & 1u) && exponent != 0x7F800000u && (b & 0x7FFFFFFFu) != 0u)
-        return __uint_as_float(((b ^ e) >> 31) ? b - 1u : b + 1u);
-    return value;
+    if (fabs(y) >= 0x1p128) return y < 0.0 ? -INFINITY : INFINITY;
+    const float f = __double2float_rz(y);
+    return (double)f == y ? f : __uint_as_float(__float_as_uint(f) | 1u);   // a NaN stays one
 }
 
-// 1 / sqrt(m) in fp64: an fp32 start (22 bits) and two Newton steps, a tenth of the instructions of a division of a
-// square root, which cost a fifth of the kernel's time
+// 1 / sqrt(m) in fp64 for m >= 1e-30: an fp32 start (22 bits) and two Newton steps, a tenth of the instructions of a
+// division of a square root, which cost a fifth of the kernel's time.  m is brought into the fp32 range first.
 __device__ __forceinline__ double inverse_sqrt(double m)
 {
-    if (!(m < 1e38)) return 1.0 / sqrt(m);   // beyond fp32, or not a number
+    const bool big = m >= 0x1p100;
+    if (big) m *= 0x1p-160;
     double r = (double)rsqrtf((float)m);
 #pragma unroll
     for (int i = 0; i < 2; ++i) r = fma(r * 0.5, fma(-m * r, r, 1.0), r);
-    return r;
+    return m == INFINITY ? 0.0 : big ? r * 0x1p-80 : r;
 }
 
 struct NormParams {
@@ -52,22 +52,37 @@ struct NormParams {
     uint8_t* scales_tc;
     int64_t x_row_bytes, r_row_bytes;
     uint32_t R, R_pad, KB, KB_pad;   // rows, rows to visit (whole records with scales_tc), blocks a row, blocks of whole chunks
-    double eps, inv_k;
+    double eps, k, inv_k;
 };
 
+// a / b, rounded once, from inv = 1 / b to about its last bit: the remainder of the rounded product is exact in a fused
+// multiply-add and corrects it (Markstein, IBM J. Res. Dev. 34, 1990); likewise the root of m from 1 / sqrt(m).  Exact
+// quotients and roots come out exactly.  b >= 0 and finite; a zero keeps its sign.  A few instructions each instead of the
+// operators' some dozens, which the one thread that needs them would wait for (300 x 4096 5.0 us, so 4.4).
+__device__ __forceinline__ double quotient(double a, double b, double inv)
+{
+    const double q = a * inv;
+    return copysign(fma(fma(-q, b, a), inv, q), a);
+}
 
-// The exact form of one value of y = h * rinv * w with rinv = rhi + rlo, rounded to odd.  h and w are read again: this runs
-// for one element in 10^5, and registers that it kept would be the common path's.
+// sqrt(sum / K + eps) of a row and its inverse; both 0 where it is infinite, which makes the quotients 0 or, of infinities, NaN
+struct NormRoot {
+    double root, inv;
+    __device__ __forceinline__ NormRoot(double sum, const NormParams& p)
+    {
+        const double m = sum == INFINITY ? sum : quotient(sum, p.k, p.inv_k) + p.eps;
+        inv = inverse_sqrt(m);
+        const double g = m * inv;
+        root = m == INFINITY ? 0.0 : fma(fma(-g, g, m), 0.5 * inv, g);
+    }
+};
+
+// y of one element in fp64, rounded to odd
 template <int DT>
-__device__ __forceinline__ float norm_exact(const uint8_t* h, const uint8_t* w, float rhi, float rlo)
+__device__ __forceinline__ float norm_exact(const uint8_t* h, const uint8_t* w, const NormRoot& row)
 {
     const float hv = unpack2<DT>(*reinterpret_cast<const uint16_t*>(h)).x, wv = unpack2<DT>(*reinterpret_cast<const uint16_t*>(w)).x;
-    const float t = hv * rhi;
-    const float t_err = fmaf(hv, rlo, fmaf(hv, rhi, -t));
-    const float v = t * wv;
-    const float v_err = fmaf(t_err, wv, fmaf(t, wv, -v));   // as much as two units in the last place of v,
-    const float y = v + v_err;                              // so the pair is brought to a nearest value and its rest
-    return round_to_odd(y, v_err - (y - v));
+    return round_to_odd(quotient((double)hv, row.root, row.inv) * (double)wv);
 }
 
 // codes of a piece times up
@@ -155,14 +170,20 @@ mx_rms_norm_kernel(const NormParams p)
         sum = part[0];
         for (uint32_t i = 1; i < blockDim.x >> 5; ++i) sum += part[i];
     }
-    const double rinv = inverse_sqrt(sum * p.inv_k + p.eps);
-    const float rhi = (float)rinv;
-    const float rlo = (float)(rinv - (double)rhi);
+    const float rinv = (float)inverse_sqrt(sum * p.inv_k + p.eps);
 
     uint8_t* codes = p.codes + (int64_t)r * (p.KB * Format<FMT>::kBytes);
+    const auto store_scale = [&](uint32_t at, uint32_t s, bool ok) {
+        const uint32_t kb = at >> 1;
+        if ((threadIdx.x & 1) != 0) return;
+        if (p.scales != nullptr && ok) p.scales[(int64_t)r * p.KB + kb] = (uint8_t)s;
+        if (p.scales_tc != nullptr && r < p.R_pad && kb < p.KB_pad) p.scales_tc[tc_offset(r, kb, p.KB_pad >> 2)] = ok ? (uint8_t)s : (uint8_t)0;
+    };
+    constexpr int kBytes = FMT == S24_MXFP4 ? 8 : 16, kWords = kBytes / 4;   // of a piece's codes
+    uint32_t todo[NC];   // of a piece: a bit per byte of codes that is not certain, the scale from bit 16, bit 24 where that is not either
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-        const uint32_t at = sub + c * tpr, kb = at >> 1;
+        const uint32_t at = sub + c * tpr;
         const bool ok = at < pieces;   // the same for the two threads of a block
         uint32_t w[8];
 #pragma unroll
@@ -172,7 +193,7 @@ mx_rms_norm_kernel(const NormParams p)
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const float2 a = unpack2<DT>(h[c][i]), b = unpack2<DT>(w[i]);
-            y[i] = make_pair(a.x, a.y) * make_pair(rhi, rhi) * make_pair(b.x, b.y);
+            y[i] = make_pair(a.x, a.y) * make_pair(rinv, rinv) * make_pair(b.x, b.y);
         }
         float m = 0.0f;
 #pragma unroll
@@ -182,50 +203,81 @@ mx_rms_norm_kernel(const NormParams p)
         }
         uint32_t amax = __float_as_uint(m);   // a NaN among them gives a NaN's bits, the largest
         amax = max(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 1));
-        const uint8_t* h_at = (p.residual != nullptr ? p.h + (int64_t)r * (p.KB * 64) : p.x + (int64_t)r * p.x_row_bytes) + at * 32;
-        const uint8_t* w_at = p.weight + at * 32;
         // a power of two too near to tell the scale, or numbers too small for fp32's own rounding; not a block of zeros
         const bool unsure = amax != 0u && (((amax + 8u) & 0x7FFFFFu) < 16u || amax <= 0x0E800000u);
-        if (__any_sync(0xFFFFFFFFu, unsure)) {
-            uint32_t exact = 0;
-            if (ok && unsure) {
-#pragma unroll 1
-                for (int e = 0; e < 16; ++e) exact = max(exact, magnitude_bits(norm_exact<DT>(h_at + 2 * e, w_at + 2 * e, rhi, rlo)));
-            }
-            exact = max(exact, __shfl_xor_sync(0xFFFFFFFFu, exact, 1));
-            if (unsure) amax = exact;
-        }
         const uint32_t s = scale_code<FMT>(amax);
         const float up = scale_up(s);
-        constexpr int kWords = FMT == S24_MXFP4 ? 2 : 4, kBits = FMT == S24_MXFP4 ? 4 : 8;
         uint32_t code[kWords], other[kWords];
         encode_piece<FMT>(y, up * (1.0f - 0x1p-21f), code);
         encode_piece<FMT>(y, up * (1.0f + 0x1p-21f), other);
-#pragma unroll
-        for (int i = 0; i < kWords; ++i) {
-            uint32_t d = ok ? (unsure ? 0xFFFFFFFFu : code[i] ^ other[i]) : 0u;
-#pragma unroll 1
-            while (d != 0u) {   // an element that the two do not agree on
-                const int e = (__ffs((int)d) - 1) / kBits;
-                const uint32_t mask = ((1u << kBits) - 1u) << (e * kBits);
-                const int at_e = 2 * (i * (32 / kBits) + e);
-                float one[8] = {norm_exact<DT>(h_at + at_e, w_at + at_e, rhi, rlo) * up, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-                const uint32_t q = FMT == S24_MXFP4 ? to_e2m1x8(one) : to_e4m3x4(one);
-                code[i] = (code[i] & ~mask) | ((q << (e * kBits)) & mask);
-                d &= ~mask;
-            }
-        }
         if (s == 255u) {
 #pragma unroll
-            for (int i = 0; i < kWords; ++i) code[i] = 0u;
+            for (int i = 0; i < kWords; ++i) code[i] = other[i] = 0u;
         }
         if (ok) {
             if constexpr (FMT == S24_MXFP4) *reinterpret_cast<uint2*>(codes + at * 8) = make_uint2(code[0], code[1]);
             else *reinterpret_cast<uint4*>(codes + at * 16) = make_uint4(code[0], code[1], code[2], code[3]);
-            if (p.scales != nullptr && (threadIdx.x & 1) == 0) p.scales[(int64_t)r * p.KB + kb] = (uint8_t)s;
         }
-        if (p.scales_tc != nullptr && (threadIdx.x & 1) == 0 && r < p.R_pad && kb < p.KB_pad)
-            p.scales_tc[tc_offset(r, kb, p.KB_pad >> 2)] = ok ? (uint8_t)s : (uint8_t)0;
+        store_scale(at, s, ok);
+        uint32_t differ = 0;
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) differ |= code[i] ^ other[i];
+        todo[c] = ok && unsure ? 1u << 24 : 0u;
+        if (ok && differ != 0u) {
+            todo[c] |= s << 16;
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) {   // which bytes are not zero: the last bit of each, brought together
+                uint32_t d = code[i] ^ other[i];
+                d |= d >> 4;
+                d |= d >> 2;
+                d |= d >> 1;
+                todo[c] |= ((d & 0x01010101u) * 0x01020408u >> 24) << (4 * i);
+            }
+        }
+    }
+
+    // What was not certain, again in fp64; h and w are read once more.  Here and not in the loop above, whose registers it
+    // would take (44 bytes of spills there).
+    uint32_t any = 0;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) any |= todo[c];
+    if (!__any_sync(0xFFFFFFFFu, any != 0u)) return;
+    const NormRoot row(sum, p);
+    const uint8_t* h_row = p.residual != nullptr ? p.h + (int64_t)r * (p.KB * 64) : p.x + (int64_t)r * p.x_row_bytes;
+#pragma unroll 1
+    for (int c = 0; c < NC; ++c) {
+        uint32_t t = todo[0];
+#pragma unroll
+        for (int i = 1; i < NC; ++i) t = c == i ? todo[i] : t;
+        const uint32_t at = sub + c * tpr;
+        const uint8_t *h_at = h_row + at * 32, *w_at = p.weight + at * 32;
+        uint32_t s = (t >> 16) & 0xFFu;
+        const bool unsure = (t >> 24) != 0u;   // the same for the two threads of a block
+        if (__any_sync(0xFFFFFFFFu, unsure)) {
+            uint32_t amax = 0;
+            if (unsure) {
+#pragma unroll 1
+                for (int e = 0; e < 16; ++e) amax = max(amax, magnitude_bits(norm_exact<DT>(h_at + 2 * e, w_at + 2 * e, row)));
+            }
+            amax = max(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 1));
+            if (unsure) {
+                s = scale_code<FMT>(amax);
+                store_scale(at, s, true);
+                t = kBytes == 16 ? 0xFFFFu : 0xFFu;
+            }
+        }
+        const float up = scale_up(s);
+        t &= 0xFFFFu;
+#pragma unroll 1
+        while (t != 0u) {
+            const int byte = __ffs((int)t) - 1, e = byte * (16 / kBytes);
+            float v[8] = {};
+            v[0] = norm_exact<DT>(h_at + 2 * e, w_at + 2 * e, row) * up;
+            if (FMT == S24_MXFP4) v[1] = norm_exact<DT>(h_at + 2 * e + 2, w_at + 2 * e + 2, row) * up;
+            const uint32_t q = s == 255u ? 0u : FMT == S24_MXFP4 ? to_e2m1x8(v) : to_e4m3x4(v);
+            codes[at * kBytes + byte] = (uint8_t)q;
+            t &= t - 1u;
+        }
     }
 }
 
@@ -290,6 +342,7 @@ extern "C" int s24_mx_rms_norm(const void* x, const void* residual, const void* 
     p.KB = (uint32_t)(K / kBlock);
     p.KB_pad = (uint32_t)(k_chunks(K) * 4);
     p.eps = eps;
+    p.k = (double)K;
     p.inv_k = 1.0 / (double)K;
     auto st = static_cast<cudaStream_t>(stream);
     if (dtype == S24_BF16) return fmt == S24_MXFP4 ? pick_norm<S24_BF16, S24_MXFP4>(p, st) : pick_norm<S24_BF16, S24_MXFP8>(p, st);

@@ -327,7 +327,8 @@ S24_API int s24_mx_scales_convert(const void* src, int from_layout, void* dst, i
  *   h = round(x + residual), y = h * weight / sqrt(mean(h^2) + eps), (codes, scales) = quantise(y).
  * h (R, K contiguous, x's type) is written only with a residual and may be the residual itself; without
  * one (NULL) h = x and the pointer is ignored.  y is not rounded before the quantisation: codes and
- * scales are those of the formula in 64 bits (values of y beyond the fp32 range count as infinite).
+ * scales are those of h / sqrt(sum(h^2) / K + eps) * weight in 64 bits (values of y from 2^128 on count as
+ * infinite).
  * x and residual have row strides ldx, ldr (elements, multiples of 16); weight is (K) of x's type
  * (S24_FP16 or S24_BF16).  K % 32 == 0, K <= S24_MX_NORM_MAX_K, eps in [1e-30, 1e30]; x, residual,
  * weight and h 32-byte aligned, codes and scales_tc 16-byte; either scale pointer may be NULL.

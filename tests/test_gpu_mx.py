@@ -490,3 +490,56 @@ def test_norm_on_exact_borders(s24, fmt, dtype):
     want_c, want_s = mxo.quantize(y, BITS[fmt])
     codes, scales, _, _ = s24.mx_rms_norm(x.to(DEV), w.to(DEV), eps=1e-30, fmt=fmt)
     assert np.array_equal(scales.cpu().numpy(), want_s) and np.array_equal(_codes(codes), want_c)
+
+
+def _check_norm(s24, x, w, eps, fmt):
+    """codes and scales against the formula in 64 bits, where values from 2^128 on count as infinite"""
+    _, y = mxo.rms_norm(x.double().numpy(), None, w.double().numpy(), eps, None)
+    want_c, want_s = mxo.quantize(np.where(np.abs(y) < 2.0 ** 128, y, np.inf), BITS[fmt])
+    codes, scales, tc, _ = s24.mx_rms_norm(x.to(DEV), w.to(DEV), eps=eps, fmt=fmt, want_tc=True)
+    assert np.array_equal(scales.cpu().numpy(), want_s), f"{(scales.cpu().numpy() != want_s).sum()} scales differ"
+    assert np.array_equal(_codes(codes), want_c), f"{(_codes(codes) != want_c).sum()} codes differ"
+    assert np.array_equal(tc.cpu().numpy(), mxo.tc_order(want_s))
+
+
+@pytest.mark.parametrize("fmt", ["mxfp8", "mxfp4"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("k", [96, 1568, 4096, 4128, 40000])
+def test_norm_keeps_ties_of_the_formula(s24, k, dtype, fmt):
+    """rows of one magnitude c: h / sqrt(mean) is exactly +-1 in 64 bits though 1 / c has no end, so y is +-w, which runs
+    through values exactly between two elements; a row with a single non-zero, and magnitudes near the end of the type"""
+    g = torch.Generator().manual_seed(k)
+    magnitudes = [3.0, 5.0, 7.0, 11.0, 100.0, 1.5 * 2.0 ** 13]
+    if dtype == torch.bfloat16:
+        magnitudes += [196608.0, 2.0 ** 100 * 1.75, 1.5 * 2.0 ** 126, 1.25 * 2.0 ** 127, 3.0 * 2.0 ** -20]
+    x = torch.where(torch.rand(len(magnitudes) + 1, k, generator=g) < 0.5, -1.0, 1.0) * torch.tensor([*magnitudes, 0.0]).unsqueeze(1)
+    x[-1, 41] = 7.0
+    w = torch.ldexp((torch.randint(16, 33, (k,), generator=g) / 16.0 + torch.randint(0, 2, (k,), generator=g) / 32.0),
+                    torch.randint(-9, 1, (k,), generator=g).int())
+    w.view(-1, 32)[::2, 7] = 2.0
+    for eps in (1e-30, 1e-12, 1e-6):
+        _check_norm(s24, x.to(dtype), w.to(dtype), eps, fmt)
+
+
+@pytest.mark.parametrize("fmt", ["mxfp8", "mxfp4"])
+@pytest.mark.parametrize("scale", [1e31, 1e38])
+def test_norm_of_very_large_rows(s24, scale, fmt):
+    """1 / sqrt(mean) is below what fp32 holds with all its bits"""
+    g = torch.Generator().manual_seed(6)
+    x = (torch.randn(1024, 4096, generator=g, dtype=torch.float64) * scale).clamp(-3.3e38, 3.3e38).to(torch.bfloat16)
+    _check_norm(s24, x, (1 + 0.3 * torch.randn(4096, generator=g)).to(torch.bfloat16), 1e-6, fmt)
+
+
+@pytest.mark.parametrize("fmt", ["mxfp8", "mxfp4"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_norm_rounds_like_the_formula_next_to_ties(s24, dtype, fmt):
+    """rows whose mean of squares is c^2 and whose elements are c / 3 and 5 c / 3: h / sqrt(mean) is a rounded third, and times
+    three times a value between two elements it is again such a value, or the double next to it"""
+    k = 1536
+    c = torch.tensor([3.0, 6.0, 12.0, 1.5, 0.75])
+    g = torch.Generator().manual_seed(8)
+    pattern = torch.tensor([1.0, 1.0, 5.0]).repeat(k // 3) / 3.0
+    x = torch.stack([pattern[torch.randperm(k, generator=g)] for _ in c]) * c.unsqueeze(1)
+    w = 3.0 * torch.ldexp((torch.randint(16, 33, (k,), generator=g) / 16.0 + torch.randint(0, 2, (k,), generator=g) / 32.0),
+                          torch.randint(-6, 1, (k,), generator=g).int())
+    _check_norm(s24, x.to(dtype), w.to(dtype), 1e-30, fmt)
