@@ -7,9 +7,13 @@
 // last bit of y into a whole step of the format wherever y lies at a border, so near one y is computed in
 // fp64.
 //   * the sum of squares is held in fp64 (squares of 16-bit values are exact there), in a fixed order;
-//   * 1 / sqrt(.) is computed once per row in fp64 and rounded to fp32;
-//   * y is first computed in fp32 (off by at most 2.5 * 2^-24 of itself) and rounded to the element type
-//     from both ends of y * (1 +- 2^-21): where the two agree, the code is certain.  About one element in
+//   * 1 / sqrt(.) is computed once per row in fp64, times 2^64, and rounded to fp32;
+//   * 2^64 y is first computed in fp32 (off by at most 2.5 * 2^-24 of itself) and rounded to the element type
+//     from both ends of y * (1 +- 2^-21): where the two agree, the code is certain.  The 2^64 stands in for
+//     fp32's range, so that h / sqrt(.) may be small beside a large weight: where 2^64 h / sqrt(.) is subnormal,
+//     2^64 y is off by at most 2^-150 times the weight, 2^-22, which is nothing in a block whose largest
+//     2^64 y is above 2^20.  Other blocks (y up to 2^-44 or from 2^64 on, zeros in a row beyond 2^80) count as
+//     not certain.  About one element in
 //     10^5 lies nearer to a border; its thread computes y again, in fp64 as the formula reads (a root and a
 //     division: a value that the formula puts exactly on a border stays there), and rounds it to fp32 to
 //     odd: an inexact y gets its last bit set, so the one rounding to the element type sees on which side
@@ -170,7 +174,7 @@ mx_rms_norm_kernel(const NormParams p)
         sum = part[0];
         for (uint32_t i = 1; i < blockDim.x >> 5; ++i) sum += part[i];
     }
-    const float rinv = (float)inverse_sqrt(sum * p.inv_k + p.eps);
+    const float rinv = (float)(inverse_sqrt(sum * p.inv_k + p.eps) * 0x1p64);
 
     uint8_t* codes = p.codes + (int64_t)r * (p.KB * Format<FMT>::kBytes);
     const auto store_scale = [&](uint32_t at, uint32_t s, bool ok) {
@@ -203,17 +207,14 @@ mx_rms_norm_kernel(const NormParams p)
         }
         uint32_t amax = __float_as_uint(m);   // a NaN among them gives a NaN's bits, the largest
         amax = max(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 1));
-        // a power of two too near to tell the scale, or numbers too small for fp32's own rounding; not a block of zeros
-        const bool unsure = amax != 0u && (((amax + 8u) & 0x7FFFFFu) < 16u || amax <= 0x0E800000u);
-        const uint32_t s = scale_code<FMT>(amax);
-        const float up = scale_up(s);
+        // a power of two too near to tell the scale, numbers outside 2^20 .. 2^128; not a block of zeros that are zeros
+        constexpr uint32_t kLow = 0x49800000u, kHigh = 0x7F800000u;
+        const bool unsure = amax != 0u ? amax - kLow >= kHigh - kLow || ((amax + 8u) & 0x7FFFFFu) < 16u : rinv < 0x1p-16f;
+        const uint32_t s = amax != 0u ? (amax >> 23) - 64u - Format<FMT>::kEmax : 0u;   // of no use where unsure
+        const float up = __uint_as_float((254u - 64u - s) << 23);                       // 2^(127 - s) of y is this of 2^64 y
         uint32_t code[kWords], other[kWords];
         encode_piece<FMT>(y, up * (1.0f - 0x1p-21f), code);
         encode_piece<FMT>(y, up * (1.0f + 0x1p-21f), other);
-        if (s == 255u) {
-#pragma unroll
-            for (int i = 0; i < kWords; ++i) code[i] = other[i] = 0u;
-        }
         if (ok) {
             if constexpr (FMT == S24_MXFP4) *reinterpret_cast<uint2*>(codes + at * 8) = make_uint2(code[0], code[1]);
             else *reinterpret_cast<uint4*>(codes + at * 16) = make_uint4(code[0], code[1], code[2], code[3]);
@@ -223,8 +224,8 @@ mx_rms_norm_kernel(const NormParams p)
 #pragma unroll
         for (int i = 0; i < kWords; ++i) differ |= code[i] ^ other[i];
         todo[c] = ok && unsure ? 1u << 24 : 0u;
-        if (ok && differ != 0u) {
-            todo[c] |= s << 16;
+        if (ok && !unsure && differ != 0u) {
+            todo[c] = s << 16;
 #pragma unroll
             for (int i = 0; i < kWords; ++i) {   // which bytes are not zero: the last bit of each, brought together
                 uint32_t d = code[i] ^ other[i];

@@ -543,3 +543,34 @@ def test_norm_rounds_like_the_formula_next_to_ties(s24, dtype, fmt):
     w = 3.0 * torch.ldexp((torch.randint(16, 33, (k,), generator=g) / 16.0 + torch.randint(0, 2, (k,), generator=g) / 32.0),
                           torch.randint(-6, 1, (k,), generator=g).int())
     _check_norm(s24, x.to(dtype), w.to(dtype), 1e-30, fmt)
+
+
+@pytest.mark.parametrize("fmt", ["mxfp8", "mxfp4"])
+@pytest.mark.parametrize("eps", [1e-30, 1e-6, 1e30])
+def test_norm_over_the_whole_range_of_bf16(s24, eps, fmt):
+    """rows and weights of every exponent that bf16 has: h / sqrt(mean) or y below and beyond what fp32 holds in between"""
+    def numbers(g, shape, low, high):
+        e = torch.rand(shape, generator=g, dtype=torch.float64) * (high - low) + low
+        return (torch.exp2(e) * torch.where(torch.rand(shape, generator=g) < 0.5, -1.0, 1.0)).to(torch.bfloat16)
+
+    g = torch.Generator().manual_seed(10)
+    k = 2048
+    for low, high in ((-133, 127), (-40, 127), (-133, -100), (-133, 0), (-70, -40), (60, 127)):
+        x = numbers(g, (32, k), low, high)
+        x[::3, ::2] = 0
+        for wlow, whigh in ((-133, 127), (100, 127), (-5, 5), (-133, -60)):
+            w = numbers(g, (k,), wlow, whigh)
+            w.view(-1, 32)[::5] = 0
+            _check_norm(s24, x, w, eps, fmt)
+
+
+@pytest.mark.parametrize("fmt", ["mxfp8", "mxfp4"])
+def test_norm_of_small_elements_beside_large_ones(s24, fmt):
+    """elements whose h / sqrt(mean) fp32 has only few bits for, or none, under weights that bring y back into its range"""
+    rows = [(2.0 ** 127, 1.0703125 * 2.0 ** -20, 2.0 ** 120), (2.0 ** 127, 1.0703125 * 2.0 ** -20, 2.0 ** 127), (2.0 ** 127, 2.0 ** -133, 1.5 * 2.0 ** 127),
+            (2.0 ** 100, 1.4375 * 2.0 ** -126, 1.75 * 2.0 ** 127), (2.0 ** 90, -2.0 ** -132, 2.0 ** 127), (1.0, 1.0703125 * 2.0 ** -126, 2.0 ** 127)]
+    for big, small, weight in rows:
+        x, w = torch.zeros(3, 64), torch.ones(64)
+        x[:2, 0], x[:, 32], x[1, 33], w[32:] = big, small, 3 * small, weight
+        _check_norm(s24, x.to(torch.bfloat16), w.to(torch.bfloat16), 1e-6, fmt)
+        _check_norm(s24, x.to(torch.bfloat16), w.to(torch.bfloat16), 1e-30, fmt)
