@@ -1015,10 +1015,7 @@ static int pick_mx(const MxOperand& a, const MxOperand& b, const MxParams& p, co
 {
     const int ktiles = (p.K + (F4 ? 255 : 127)) / (F4 ? 256 : 128);
     if (cfg != nullptr && (cfg->bm != 0 || cfg->bn != 0 || cfg->split != 0)) {
-        const int few = p.M < p.N ? p.M : p.N, lng = p.M < p.N ? p.N : p.M, split = cfg->split;
-        if (split != 0 && (few > 8192 || lng > 65535 * 128 || (split != 1 && split != 2 && split != 4 && split != 8)))
-            return fail(S24_ERR_UNSUPPORTED, "mx_matmul: K can be split 1, 2, 4 or 8 ways, with at most 8192 rows on one side (got %d)", split);
-        MxPlan plan = {0.0, cfg->bm, cfg->bn, split};
+        MxPlan plan = {0.0, cfg->bm, cfg->bn, cfg->split};
         if (plan.bm == 0) plan.bm = plan.bn == 256 || p.M > 128 ? 256 : 128;
         if (plan.bn == 0) plan.bn = 128;
         return launch_plan<F4>(a, b, p, plan, stream);
@@ -1054,6 +1051,13 @@ extern "C" int s24_mx_matmul(const void* a, const void* a_scales, const void* b,
     if (!aligned(a, step_a) || !aligned(b, step_b) || !aligned(a_scales, 16) || !aligned(b_scales, 16) || !aligned(C, esz))
         return fail(S24_ERR_INVALID_ARG, "mx_matmul: codes must be %lld / %lld-byte aligned, scales 16-byte and C by its element", (long long)step_a,
                     (long long)step_b);
+    if (cfg != nullptr && cfg->split != 0) {
+        const int64_t few = M < N ? M : N, lng = M < N ? N : M;
+        const int split = cfg->split;
+        if (cfg->bm != 0 || cfg->bn != 0) return fail(S24_ERR_UNSUPPORTED, "mx_matmul: a split of K has tiles of its own (got %d x %d with it)", cfg->bm, cfg->bn);
+        if (few > 8192 || lng > 65535 * 128 || (split != 1 && split != 2 && split != 4 && split != 8))
+            return fail(S24_ERR_UNSUPPORTED, "mx_matmul: K can be split 1, 2, 4 or 8 ways, with at most 8192 rows on one side (got %d)", split);
+    }
     int* status = status_word_address();
     if (status == nullptr) return fail(S24_ERR_CUDA, "mx_matmul: cannot resolve the device status word");
 

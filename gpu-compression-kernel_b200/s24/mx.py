@@ -215,7 +215,8 @@ def mx_matmul(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_scales
 
     a and b are codes of either format, their scales in tensor-core order (`want_tc=True`, or mx_scales_convert);
     K must be a multiple of 128 where the formats differ.  `out` (2-dimensional, of `out_dtype`) must not
-    overlap the operands.  As with every product of the library, make the first call on a device before a stream
+    overlap the operands.  `manual_config` has a tile ("BM" and "BN": 256 x 256, 256 x 128 or 128 x 128) or "SPLIT", the
+    number of CTAs that share K (1, 2, 4 or 8; 1 where K has fewer steps than that).  As with every product of the library, make the first call on a device before a stream
     capture.
     """
     fa, M, K = _codes_of(a)

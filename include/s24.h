@@ -137,7 +137,8 @@ typedef struct s24_tile_cfg {
     int stages;    /* reserved, ignored: every tile shape has one ring depth (512x224: 3, 256x256: 4,
                       256x128: 6, 128x128: 4 stages of K = 128) that fills the 227 KB of shared memory */
     int split;     /* s24_mx_matmul only, others ignore it: number of CTAs that share K (1, 2, 4 or 8), on tiles of 128 x 128
-                      or less, with at most 8192 rows on one side; 0 = auto */
+                      or less, with bm = bn = 0 and at most 8192 rows on one side; 0 = auto.  A K of fewer steps than that (of
+                      256 elements where both operands are 4-bit, of 128 otherwise) is not split */
 } s24_tile_cfg;
 
 S24_API int s24_version(void);

@@ -574,3 +574,19 @@ def test_norm_of_small_elements_beside_large_ones(s24, fmt):
         x[:2, 0], x[:, 32], x[1, 33], w[32:] = big, small, 3 * small, weight
         _check_norm(s24, x.to(torch.bfloat16), w.to(torch.bfloat16), 1e-6, fmt)
         _check_norm(s24, x.to(torch.bfloat16), w.to(torch.bfloat16), 1e-30, fmt)
+
+
+@pytest.mark.parametrize("fa,fb", PAIRS)
+@pytest.mark.parametrize("m,n", [(1, 130), (7, 1000), (33, 257), (130, 70), (300, 200)])
+def test_product_with_k_really_split(s24, m, n, fa, fb):
+    """as many k-tiles as CTAs that share them, and a few more; a tile with it is refused"""
+    for k in (2048, 2560):
+        a, sa, va = _operand(s24, m, k, fa, m + k, True)
+        b, sb, vb = _operand(s24, n, k, fb, n + k + 1, True)
+        want = torch.from_numpy(va) @ torch.from_numpy(vb).t()
+        for split in SPLITS:
+            got = s24.mx_matmul(a, sa, b, sb, out_dtype=torch.float32, manual_config=split)
+            assert torch.equal(got.cpu().double(), want), (k, split)
+    with pytest.raises(s24.S24Error, match="tiles of its own"):
+        s24.mx_matmul(a, sa, b, sb, manual_config={"BM": 256, "BN": 128, "SPLIT": 2})
+    assert s24.lib().s24_device_status(None) == 0

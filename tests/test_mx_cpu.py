@@ -160,3 +160,20 @@ def test_c_entry_refusals_need_no_gpu(s24):
     assert m(p, p, p, p, p, 4, 4, 64, 32, 32, 4, 0, 0, 2, None, None) == I
     assert m(p, p, p, p, p, 1 << 40, 4, 64, 32, 32, 4, 0, 0, 1, None, None) == S
     assert m(None, None, None, None, None, 0, 4, 64, 32, 32, 4, 0, 0, 1, None, None) == _lib.OK
+
+
+def test_split_refusals_need_no_gpu(s24):
+    """a split that is not a power of two up to 8, that a side has too many rows for, or that comes with a tile"""
+    from s24 import _lib
+    p = ctypes.cast(ctypes.create_string_buffer(4096 + 64), ctypes.c_void_p)
+    p = ctypes.c_void_p((p.value + 63) & ~63)
+
+    def product(m, n, *cfg):
+        return _lib.lib().s24_mx_matmul(p, p, p, p, p, m, n, 1024, 512, 512, n, 0, 0, 1, ctypes.byref(_lib.TileCfg(*cfg)), None)
+
+    for split in (3, 16, -1):
+        assert product(4, 4, 0, 0, 0, split) == _lib.ERR_UNSUPPORTED
+    assert product(8193, 8193, 0, 0, 0, 2) == _lib.ERR_UNSUPPORTED
+    assert product(4, 65535 * 128 + 1, 0, 0, 0, 2) == _lib.ERR_UNSUPPORTED
+    for bm, bn in ((256, 256), (256, 0), (0, 128), (128, 128)):
+        assert product(4, 4, bm, bn, 0, 2) == _lib.ERR_UNSUPPORTED and "tiles of its own" in _lib.last_error()
