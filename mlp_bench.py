@@ -26,7 +26,7 @@ import torch.distributed as dist
 
 sys.path.insert(0, str(Path(__file__).resolve().parent / "gpu-compression-kernel_b200"))
 import s24  # noqa: E402
-from s24.multi import NShardedSpmm  # noqa: E402
+from s24.multi import NShardedSpmm, shard_bounds  # noqa: E402
 
 M, K, N = 28672, 8192, 65536
 
@@ -44,11 +44,13 @@ def main():
         dist.init_process_group("nccl", device_id=dev, timeout=datetime.timedelta(seconds=300))
     g = torch.Generator(device=dev).manual_seed(5000)                    # same W on every rank
     W = (0.02 * torch.randn(M, K, generator=g, device=dev, dtype=torch.float32)).to(torch.bfloat16)
-    vals, _, tc = s24.prune_compress(W, want_ref=False, want_tc=True)    # compressed redundantly, no broadcast
-    W4, _, W4_tc = s24.mx_quantize(W, "mxfp4", want_rows=False, want_tc=True) if args.mx else (None, None, None)
+    if args.mx:                                                          # compressed redundantly, no broadcast
+        W4, _, W4_tc = s24.mx_quantize(W, "mxfp4", want_rows=False, want_tc=True)
+    else:
+        vals, _, tc = s24.prune_compress(W, want_ref=False, want_tc=True)
+        op = NShardedSpmm(vals, tc)
     del W
-    op = NShardedSpmm(vals, tc)
-    n0, n1 = op.local_columns(N)
+    n0, n1 = shard_bounds(N, world, rank)
     gx = torch.Generator(device=dev).manual_seed(5001 + rank)
     X = torch.randn(K, n1 - n0, generator=gx, device=dev, dtype=torch.float32).to(torch.bfloat16)
     if args.mx:
@@ -83,7 +85,6 @@ def main():
             return s24.mx_matmul(codes, scales, W4, W4_tc)
 
         ms = timed(mx_step, args.steps)
-        op.close()
         if rank == 0:
             print(json.dumps({"workload": f"X {N}x{K} bf16 -> mxfp8 . (W {M}x{K} mxfp4)^T, tokens sharded x{world}", "n_gpus": world,
                               "mx": {"ms": ms, "tflops": flops / ms / 1e9}}), flush=True)

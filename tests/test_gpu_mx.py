@@ -590,3 +590,25 @@ def test_product_with_k_really_split(s24, m, n, fa, fb):
     with pytest.raises(s24.S24Error, match="tiles of its own"):
         s24.mx_matmul(a, sa, b, sb, manual_config={"BM": 256, "BN": 128, "SPLIT": 2})
     assert s24.lib().s24_device_status(None) == 0
+
+
+def test_mlp_bench_in_microscaled_formats_makes_no_sparse_operand(s24, monkeypatch, capsys):
+    """a small case of the benchmark's --mx form, with the sparse path out of reach"""
+    import json
+    import sys
+
+    import mlp_bench
+
+    def out_of_reach(*args, **kwargs):
+        raise AssertionError("called for a run without a sparse operand")
+
+    for name, value in (("M", 512), ("K", 256), ("N", 384)):
+        monkeypatch.setattr(mlp_bench, name, value)
+    monkeypatch.setattr(s24, "prune_compress", out_of_reach)
+    monkeypatch.setattr(mlp_bench, "NShardedSpmm", out_of_reach)
+    for name in ("RANK", "WORLD_SIZE", "LOCAL_RANK"):
+        monkeypatch.delenv(name, raising=False)
+    monkeypatch.setattr(sys, "argv", ["mlp_bench.py", "--mx", "--steps", "2"])
+    mlp_bench.main()
+    line = json.loads(capsys.readouterr().out.splitlines()[-1])
+    assert line["n_gpus"] == 1 and line["mx"]["ms"] > 0
