@@ -113,7 +113,9 @@ constexpr int kStoreWarpBytes = 32 * kStorePitch * 4;
 // 8192^3 4-bit 210 / 210 / 208 / 207 us, 8-bit 438 / 428 / 421 / 468, 4001 x 28672 x 8192 700 / 689 / 682 / 682,
 // 16384^3 4-bit 1639 / 1577 / 1550 / 1746 (with 16 now 200, 409, 674 and 1518).
 constexpr int kMxGroupM = 16;
-constexpr int kMxPart = 128;   // a tile's columns start on a record of B's scales
+// Parts of a tile start on whole records of B's scales; from a record's middle they would be read two tensor-memory columns
+// further on, which is not built.
+constexpr int kMxPart = 128;
 
 struct MxTile {
     int m, col, width;   // row tile, first column, columns the MMA makes: a multiple of 64; none: nothing left to do
@@ -173,13 +175,6 @@ struct MxCfg {
     static_assert(8 * (2 * ST + 2) + 16 <= 256, "barrier block");
 };
 
-__device__ __forceinline__ void store_sector(void* p, const uint32_t* q)
-{
-    asm volatile("st.global.L1::no_allocate.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(q[0]), "r"(q[1]), "r"(q[2]), "r"(q[3]),
-                 "r"(q[4]), "r"(q[5]), "r"(q[6]), "r"(q[7])
-                 : "memory");
-}
-
 __device__ __forceinline__ uint32_t ld_shared_u32(uint32_t addr)
 {
     uint32_t v;
@@ -198,7 +193,7 @@ __device__ __forceinline__ void mx_store_aligned(const MxParams& p, int row0, in
 #pragma unroll
         for (int i = 0; i < 64; i += 8) {
             if (col + i + 8 <= p.N) {
-                store_sector(c + i, &r[i]);
+                mx::store32(c + i, &r[i]);
             } else {
 #pragma unroll
                 for (int k = 0; k < 8; ++k)
@@ -214,7 +209,7 @@ __device__ __forceinline__ void mx_store_aligned(const MxParams& p, int row0, in
 #pragma unroll
         for (int k = 0; k < 8; ++k) q[k] = pack2(__uint_as_float(r[i + 2 * k]), __uint_as_float(r[i + 2 * k + 1]), p.out == S24_BF16);
         if (col + i + 16 <= p.N) {
-            store_sector(c + i, q);
+            mx::store32(c + i, q);
         } else {
 #pragma unroll
             for (int k = 0; k < 16; ++k)
@@ -818,6 +813,20 @@ static int make_scale_map(CUtensorMap* map, const MxOperand& o, int64_t K, int c
 // 64 of the 128 bytes it covers (measured; the padding is not written either)
 static uint32_t code_tx(const MxOperand& o, bool both4, int rows) { return (uint32_t)rows * ((both4 || o.fmt == S24_MXFP8) ? 128u : 64u); }
 
+// the opt-in to more than 48 KB of shared memory, once per kernel and device
+template <auto* Kernel>
+static int allow_smem(int bytes)
+{
+    static bool opted_in[64] = {false};
+    int dev = 0;
+    int rc = check_cuda(cudaGetDevice(&dev), "cudaGetDevice");
+    if (rc) return rc;
+    if (dev >= 0 && dev < 64 && opted_in[dev]) return S24_OK;
+    rc = check_cuda(cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), "cudaFuncSetAttribute(max dynamic shared memory)");
+    if (rc == S24_OK && dev >= 0 && dev < 64) opted_in[dev] = true;
+    return rc;
+}
+
 template <class Cfg>
 static int launch_mx(const MxOperand& a, const MxOperand& b, MxParams p, cudaStream_t stream)
 {
@@ -829,18 +838,8 @@ static int launch_mx(const MxOperand& a, const MxOperand& b, MxParams p, cudaStr
     if (rc) return rc;
     p.tx_bytes = code_tx(a, Cfg::kF4, 128) + Cfg::kSABytes + Cfg::kSBBytes;
     p.tx_box = code_tx(b, Cfg::kF4, Cfg::kBox);
-    {
-        static bool opted_in[64] = {false};
-        int dev = 0;
-        rc = check_cuda(cudaGetDevice(&dev), "cudaGetDevice");
-        if (rc) return rc;
-        if (dev < 0 || dev >= 64 || !opted_in[dev]) {
-            rc = check_cuda(cudaFuncSetAttribute(mx_matmul_kernel<Cfg>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes),
-                            "cudaFuncSetAttribute(max dynamic shared memory)");
-            if (rc) return rc;
-            if (dev >= 0 && dev < 64) opted_in[dev] = true;
-        }
-    }
+    rc = allow_smem<mx_matmul_kernel<Cfg>>(Cfg::kSmemBytes);
+    if (rc) return rc;
     const int64_t tiles = (int64_t)((p.M + 128 * Cfg::kG - 1) / (128 * Cfg::kG)) * ((p.N + Cfg::kBN - 1) / Cfg::kBN);
     if (tiles > 0x7FFFFFFFll / kMxGroupM) return fail(S24_ERR_SHAPE, "mx_matmul: too many output tiles");
     int units = sm_count() / Cfg::kG;
@@ -895,18 +894,8 @@ static int launch_few_cfg(const MxOperand& a, const MxOperand& b, FewParams p, i
     if (!rc) rc = make_scale_map(&tm_sb, b, K, Cfg::kChunks, 1, "scales of the few rows");
     if (rc) return rc;
     p.tx_bytes = code_tx(a, Cfg::kF4, 128) + code_tx(b, Cfg::kF4, Cfg::kNT) + 2 * Cfg::kSBytes;
-    {
-        static bool opted_in[64] = {false};
-        int dev = 0;
-        rc = check_cuda(cudaGetDevice(&dev), "cudaGetDevice");
-        if (rc) return rc;
-        if (dev < 0 || dev >= 64 || !opted_in[dev]) {
-            rc = check_cuda(cudaFuncSetAttribute(mx_matmul_few_kernel<Cfg>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes),
-                            "cudaFuncSetAttribute(max dynamic shared memory)");
-            if (rc) return rc;
-            if (dev >= 0 && dev < 64) opted_in[dev] = true;
-        }
-    }
+    rc = allow_smem<mx_matmul_few_kernel<Cfg>>(Cfg::kSmemBytes);
+    if (rc) return rc;
     const int tiles = (p.n_long + 127) / 128, across = (p.n_few + Cfg::kNT - 1) / Cfg::kNT;
     return check_cuda(mx::launch_overlapped(mx_matmul_few_kernel<Cfg>, dim3((unsigned)split, (unsigned)tiles, (unsigned)across), kFewThreads, Cfg::kSmemBytes, (unsigned)split, stream,
                                             tm_a, tm_b, tm_sa, tm_sb, p),
