@@ -944,8 +944,8 @@ static int run_few(const MxOperand& a, const MxOperand& b, const MxParams& p, in
 // last epilogue), one per k-tile and pass over the SMs, and one per further pass; a split of K a fixed part, one per
 // k-tile of a CTA, more where SMs have two, and the sum over the cluster.  The constants are fitted to 220 shapes drawn
 // over 1 to 4096 rows, 64 to 16384 columns and K of 256 to 16384 in three pairs of formats, each timed with every tile and
-// split; on 220 others what the model picks takes 1.02 times the best of them on average, 1.24 at worst.  Examples (tiles
-// 256 x 256, 256 x 128, 128 x 128, then 1, 2, 4, 8 CTAs sharing K): 8192^3 4-bit 183 / 235 / 287 and 341 to 1160 us;
+// split; on 216 others (profiles/mx_tile_choice.csv) what the model picks takes 1.02 times the best of them on average, 1.31
+// at worst.  Examples (tiles 256 x 256, 256 x 128, 128 x 128, then 1, 2, 4, 8 CTAs sharing K): 8192^3 4-bit 183 / 235 / 287 and 341 to 1160 us;
 // 543 x 1792 x 1792 8-by-4-bit 9.6 / 6.6 / 6.2, 12.1 / 12.1 / 10.0 / 20.5; 65 x 561 x 12032 41.8 / 25.0 / 24.4, 36.7 / 22.7 /
 // 13.1 / 8.6; 1 x 4096 x 4096 15 / 16 / 10, 7.0 / 5.2 / 4.6 / 5.2; 4 x 28672 x 8192 54 / 74 / 59, 22.2 / 27.4 / 32.9 / 45.
 struct MxPlan {

@@ -110,9 +110,12 @@ __device__ __forceinline__ void encode_piece(const Pair (&y)[8], float up, uint3
 // all, 32 bytes each, so that a warp's accesses are whole lines.  The row stays in registers between the sum and the
 // quantisation: x and the residual are read once.
 //
-// What bounds it: with a residual the 7.03 bytes an element (8 bits out), without one the instructions, about 14 an
-// element.  Measured, 8192 x 8192 bf16 with a residual: a block per thread 117 us, an eighth of a block (8 elements) per
-// thread 74 to 80 us with 22 to 28 instructions an element; 4099 x 6144 fp16 to 4 bits 34, 25 to 27 us.
+// What bounds it: with a residual the 7.03 bytes an element (8 bits out): 8192 x 8192 bf16 71.5 us, the measured
+// copy rate.  Without one neither bytes nor a pipe: 4099 x 6144 fp16 to 4 bits is 18.6 us for 9.9 us of bytes, at 16
+// instructions an element, 52 % of the issue slots (63 % while an SM is active) and no pipe above 35 %.  A CTA's loads, its
+// sum and its encoding follow one another, and what warps wait for most is the loads.  The second rounding and what
+// follows from it are 11 %.  Steps, 8192 x 8192 with a residual: a block per thread 117 us, an eighth of a block (8 elements)
+// per thread 74 to 80, half a block 72.
 template <int DT, int FMT, int TPR, int NC>
 __global__ void __launch_bounds__(TPR == 0 ? 1024 : 128, TPR == 0 ? 1 : 8)
 mx_rms_norm_kernel(const NormParams p)

@@ -123,7 +123,9 @@ mx_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restric
     }
 }
 
-// One thread per scale of the destination; positions of tensor-core order outside the matrix get 0.
+// One thread per scale of the destination; positions of tensor-core order outside the matrix get 0.  Bound by its byte
+// accesses: 28672 x 8192 31 us either way for 2.3 us of bytes.  It runs once per weight, when a checkpoint is loaded; what
+// runs in a step writes the order that it needs itself.
 template <bool TO_TC>
 __global__ void __launch_bounds__(kQuantThreads)
 mx_scales_convert_kernel(const uint8_t* __restrict__ src, uint8_t* __restrict__ dst, uint32_t R, uint32_t KB, uint32_t total)
