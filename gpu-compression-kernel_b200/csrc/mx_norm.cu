@@ -12,8 +12,8 @@
 //     from both ends of y * (1 +- 2^-21): where the two agree, the code is certain.  The 2^64 stands in for
 //     fp32's range, so that h / sqrt(.) may be small beside a large weight: where 2^64 h / sqrt(.) is subnormal,
 //     2^64 y is off by at most 2^-150 times the weight, 2^-22, which is nothing in a block whose largest
-//     2^64 y is above 2^20.  Other blocks (y up to 2^-44 or from 2^64 on, zeros in a row beyond 2^80) count as
-//     not certain.  About one element in
+//     2^64 y is above 2^20; with a row's root below 2^57 none is subnormal, and 2^-100 does.  Other blocks
+//     (y below that or from 2^64 on, zeros in a row beyond 2^80) count as not certain.  About one element in
 //     10^5 lies nearer to a border; its thread computes y again, in fp64 as the formula reads (a root and a
 //     division: a value that the formula puts exactly on a border stays there), and rounds it to fp32 to
 //     odd: an inexact y gets its last bit set, so the one rounding to the element type sees on which side
@@ -111,7 +111,7 @@ __device__ __forceinline__ void encode_piece(const Pair (&y)[8], float up, uint3
 // quantisation: x and the residual are read once.
 //
 // What bounds it: with a residual the 7.03 bytes an element (8 bits out): 8192 x 8192 bf16 71.5 us, the measured
-// copy rate.  Without one neither bytes nor a pipe: 4099 x 6144 fp16 to 4 bits is 18.6 us for 9.9 us of bytes, at 16
+// copy rate.  Without one neither bytes nor a pipe: 4099 x 6144 fp16 to 4 bits is 18.8 us for 9.9 us of bytes, at 16
 // instructions an element, 52 % of the issue slots (63 % while an SM is active) and no pipe above 35 %.  A CTA's loads, its
 // sum and its encoding follow one another, and what warps wait for most is the loads.  The second rounding and what
 // follows from it are 11 %.  Steps, 8192 x 8192 with a residual: a block per thread 117 us, an eighth of a block (8 elements)
@@ -179,6 +179,9 @@ mx_rms_norm_kernel(const NormParams p)
     }
     const float rinv = (float)(inverse_sqrt(sum * p.inv_k + p.eps) * 0x1p64);
 
+    // the largest 2^64 y of a block has to be above 2^20, or above 2^-100 where h of 2^-133 still makes a normal number
+    const uint32_t low = rinv < 128.0f ? 0x49800000u : 0x0D800000u;
+
     uint8_t* codes = p.codes + (int64_t)r * (p.KB * Format<FMT>::kBytes);
     const auto store_scale = [&](uint32_t at, uint32_t s, bool ok) {
         const uint32_t kb = at >> 1;
@@ -210,10 +213,9 @@ mx_rms_norm_kernel(const NormParams p)
         }
         uint32_t amax = __float_as_uint(m);   // a NaN among them gives a NaN's bits, the largest
         amax = max(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 1));
-        // a power of two too near to tell the scale, numbers outside 2^20 .. 2^128; not a block of zeros that are zeros
-        constexpr uint32_t kLow = 0x49800000u, kHigh = 0x7F800000u;
-        const bool unsure = amax != 0u ? amax - kLow >= kHigh - kLow || ((amax + 8u) & 0x7FFFFFu) < 16u : rinv < 0x1p-16f;
-        const uint32_t s = amax != 0u ? (amax >> 23) - 64u - Format<FMT>::kEmax : 0u;   // of no use where unsure
+        // a power of two too near to tell the scale, numbers outside low .. 2^128; not a block of zeros that are zeros
+        const bool unsure = amax != 0u ? amax - low >= 0x7F800000u - low || ((amax + 8u) & 0x7FFFFFu) < 16u : rinv < 0x1p-16f;
+        const uint32_t s = (uint32_t)max((int)(amax >> 23) - 64 - Format<FMT>::kEmax, 0);   // of no use where unsure
         const float up = __uint_as_float((254u - 64u - s) << 23);                       // 2^(127 - s) of y is this of 2^64 y
         uint32_t code[kWords], other[kWords];
         encode_piece<FMT>(y, up * (1.0f - 0x1p-21f), code);
